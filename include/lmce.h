@@ -47,7 +47,7 @@ enum {
   LMCE_ERR_WORKSPACE = 6         /* workspace too small */
 };
 
-enum { LMCE_DTYPE_F16 = 0, LMCE_DTYPE_BF16 = 1 };
+enum { LMCE_DTYPE_F16 = 0, LMCE_DTYPE_BF16 = 1, LMCE_DTYPE_F32 = 2 /* gradients to clip only */ };
 
 /* Per-token partial softmax statistics, 24 bytes:
  *   m    running max of the logits (logits rounded to the input dtype)
@@ -262,6 +262,50 @@ LMCE_API int lmce_embedding_grad_add(const void* d_embed, const int64_t* token_i
 LMCE_API int lmce_embedding_lookup(const void* weight, const int64_t* token_ids, int64_t n_tokens,
                                    int64_t hidden_dim, int64_t vocab_local, int64_t vocab_offset, void* out,
                                    void* stream);
+
+/* -------------------------------------------- residual add + RMSNorm */
+
+/* Residual addition with its RMSNorm, the front of a decoder block's sub-layer (the
+ * reference fuses the pair in rms_norm_fwd, kernels.py:125-164):
+ *   s = dtype(x + residual),  rstd = 1/sqrt(mean(s^2) + eps),  y = dtype(s * rstd * weight)
+ * with fp32 sums and one rounding of y. residual may be null: s = x, and s_out is not used.
+ *   x, residual, s_out, y_out  [n_rows, hidden_dim] dtype, contiguous, 16-byte aligned
+ *   weight [hidden_dim] dtype; rstd_out [n_rows] fp32 (nullable), for the backward
+ * hidden_dim: a multiple of 8, at most 32768. */
+LMCE_API int lmce_add_rmsnorm(const void* x, const void* residual, const void* weight, float eps, int64_t n_rows,
+                              int64_t hidden_dim, int dtype, void* s_out, void* y_out, float* rstd_out,
+                              void* stream);
+
+/* The same with y in e4m3 and one scale per row, the operand of 8-bit products:
+ *   scale = max|s * rstd * weight| / 448 (1 for a row of zeros),  q = e4m3(s * rstd * weight / scale)
+ *   q_out [n_rows, hidden_dim] bytes; scale_out [n_rows] fp32 */
+LMCE_API int lmce_add_rmsnorm_e4m3(const void* x, const void* residual, const void* weight, float eps,
+                                   int64_t n_rows, int64_t hidden_dim, int dtype, void* s_out, void* q_out,
+                                   float* scale_out, void* stream);
+
+LMCE_API size_t lmce_add_rmsnorm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim);
+
+/* Backward of lmce_add_rmsnorm (reference: rms_norm_bwd, kernels.py:167-199, which has no
+ * weight gradient). s is s_out (or x without residual). d_y and d_s are the gradients of y and
+ * s (each nullable: zero); d_x is the gradient of x and of residual alike (nullable);
+ * d_weight [hidden_dim] dtype (nullable; the workspace is used only with it). Deterministic. */
+LMCE_API int lmce_add_rmsnorm_backward(const void* d_y, const void* d_s, const void* s, const void* weight,
+                                       const float* rstd, int64_t n_rows, int64_t hidden_dim, int dtype, void* d_x,
+                                       void* d_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* -------------------------------------------------- gradient clipping */
+
+LMCE_API size_t lmce_clip_grad_workspace_bytes(int64_t count);
+
+/* total_norm = sqrt(sum over all gradients of sum g^2); where max_norm / (total_norm + 1e-6) is
+ * below 1 (or not a number) every gradient is multiplied by it in place. fp64 sums, the same
+ * bits for the same gradients. `grads`, `numels` and `dtypes` are host arrays read during the
+ * call (nothing is kept, the launches may be captured): device pointers aligned to their
+ * element, sizes in elements (0: skipped), LMCE_DTYPE_* (fp32 included). Gradients may not
+ * overlap. max_norm = infinity only measures. total_norm: device fp32 scalar. count at most 2^20. */
+LMCE_API int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int64_t count,
+                                 float max_norm, float* total_norm, void* workspace, size_t workspace_bytes,
+                                 void* stream);
 
 /* ----------------------------------------------- no-allocation forward */
 

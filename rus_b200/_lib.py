@@ -22,6 +22,7 @@ LMCE_ERR_WORKSPACE = 6
 
 LMCE_DTYPE_F16 = 0
 LMCE_DTYPE_BF16 = 1
+LMCE_DTYPE_F32 = 2  # gradients to clip only
 
 PART_BYTES = 24  # sizeof(lmce_part)
 
@@ -89,6 +90,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lmce_embedding_lookup": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "lmce_rmsnorm_pack": (_int, [_vp, _vp, ctypes.c_float, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "lmce_rmsnorm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
+    "lmce_add_rmsnorm": (_int, [_vp, _vp, _vp, ctypes.c_float, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
+    "lmce_add_rmsnorm_e4m3": (_int, [_vp, _vp, _vp, ctypes.c_float, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
+    "lmce_add_rmsnorm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "lmce_add_rmsnorm_backward": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "lmce_clip_grad_workspace_bytes": (ctypes.c_size_t, [_i64]),
+    "lmce_clip_grad_norm": (_int, [_vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp]),
     "lmce_dx_finalize": (_int, [_vp, _i64, _i64, _int, _vp, _vp]),
     "lmce_selftest_wait_timeout": (_int, [ctypes.c_uint64, _vp]),
     "lmce_launch_count": (ctypes.c_uint64, []),

@@ -1435,3 +1435,5 @@ extern "C" int lmce_forward_noalloc(const void* hidden, const void* weight, cons
   return lmce_stats_finish(recs, parts, parts, 1, labels, n_tokens, num_items_dev, num_items, lse, nll, entropy,
                            argmax, loss, denom, stream);
 }
+
+#include "lmce_layer_capi.cuh"
