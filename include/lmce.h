@@ -271,7 +271,7 @@ LMCE_API int lmce_embedding_lookup(const void* weight, const int64_t* token_ids,
  * with fp32 sums and one rounding of y. residual may be null: s = x, and s_out is not used.
  *   x, residual, s_out, y_out  [n_rows, hidden_dim] dtype, contiguous, 16-byte aligned
  *   weight [hidden_dim] dtype; rstd_out [n_rows] fp32 (nullable), for the backward
- * hidden_dim: a multiple of 8, at most 32768. */
+ * hidden_dim: a multiple of 8, at most 16384. */
 LMCE_API int lmce_add_rmsnorm(const void* x, const void* residual, const void* weight, float eps, int64_t n_rows,
                               int64_t hidden_dim, int dtype, void* s_out, void* y_out, float* rstd_out,
                               void* stream);
@@ -292,6 +292,43 @@ LMCE_API size_t lmce_add_rmsnorm_bwd_workspace_bytes(int64_t n_rows, int64_t hid
 LMCE_API int lmce_add_rmsnorm_backward(const void* d_y, const void* d_s, const void* s, const void* weight,
                                        const float* rstd, int64_t n_rows, int64_t hidden_dim, int dtype, void* d_x,
                                        void* d_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------- gated projection */
+
+enum { LMCE_ACT_SILU = 0, LMCE_ACT_GELU_TANH = 1 };
+
+/* The gated projection of a feed-forward block in one kernel (the reference: two cuBLAS
+ * products and swiglu_fwd, kernels.py:355-400):
+ *   h = act(x . w_gate^T) * (x . w_up^T),  fp32 accumulation and activation, one rounding
+ *   x [n_rows, hidden_dim], w_gate and w_up [ffn_dim, hidden_dim], h_out [n_rows, ffn_dim]
+ * dtype, contiguous, 16-byte aligned; hidden_dim and ffn_dim multiples of 64. `saved`
+ * (nullable) receives what the backward needs, lmce_gated_saved_bytes bytes. */
+LMCE_API size_t lmce_gated_saved_bytes(int64_t n_rows, int64_t ffn_dim);
+LMCE_API int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64_t n_rows,
+                               int64_t hidden_dim, int64_t ffn_dim, int dtype, int act, void* h_out, void* saved,
+                               void* stream);
+
+/* The same on e4m3 operands with fp32 scales (no backward): x stands for x * x_scale[row], a
+ * weight for w * scale[feature]. hidden_dim a multiple of 128, ffn_dim of 64; out_dtype is the
+ * type of h_out. The weights' scales are 16-byte aligned. */
+LMCE_API int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const void* w_gate,
+                                    const float* gate_scale, const void* w_up, const float* up_scale,
+                                    int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int out_dtype, int act,
+                                    void* h_out, void* stream);
+
+LMCE_API size_t lmce_gated_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int want_dx,
+                                               int n_weights);
+
+/* Backward of lmce_gated_linear (the reference: swiglu_bwd, kernels.py:403-446, and two cuBLAS
+ * products; its weights are frozen):
+ *   dg = dtype(d_h * u * act'(g)), du = dtype(d_h * act(g)),
+ *   d_x = dg . w_gate + du . w_up, d_gate = dg^T . x, d_up = du^T . x
+ * Each of d_x, d_gate and d_up may be null (not all). The workspace is 256-byte aligned,
+ * lmce_gated_bwd_workspace_bytes(..., d_x != null, number of weight gradients). Deterministic. */
+LMCE_API int lmce_gated_backward(const void* d_h, const void* saved, const void* x, const void* w_gate,
+                                 const void* w_up, int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int dtype,
+                                 int act, void* d_x, void* d_gate, void* d_up, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 
 /* -------------------------------------------------- gradient clipping */
 

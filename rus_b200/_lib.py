@@ -24,6 +24,9 @@ LMCE_DTYPE_F16 = 0
 LMCE_DTYPE_BF16 = 1
 LMCE_DTYPE_F32 = 2  # gradients to clip only
 
+LMCE_ACT_SILU = 0
+LMCE_ACT_GELU_TANH = 1
+
 PART_BYTES = 24  # sizeof(lmce_part)
 
 
@@ -96,6 +99,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lmce_add_rmsnorm_backward": (
         _int,
         [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "lmce_gated_saved_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "lmce_gated_linear": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp]),
+    "lmce_gated_linear_e4m3": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp],
+    ),
+    "lmce_gated_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int, _int]),
+    "lmce_gated_backward": (
+        _int,
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
     ),
     "lmce_clip_grad_workspace_bytes": (ctypes.c_size_t, [_i64]),
     "lmce_clip_grad_norm": (_int, [_vp, _vp, _vp, _i64, ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp]),

@@ -1,0 +1,826 @@
+// Gated projection of a feed-forward block, forward and backward:
+//   h = act(x . Wg^T) * (x . Wu^T)                  x [N, H], Wg and Wu [F, H], h [N, F]
+//   act(g) = g * sig(v): silu v = g; gelu (tanh form) v = 2 sqrt(2/pi) (g + 0.044715 g^3),
+//   which is 0.5 g (1 + tanh(v / 2)) without the cancellation of 1 + tanh
+// (the reference runs two cuBLAS products and the kernels swiglu_fwd / swiglu_bwd,
+// solution/kernels.py:355-446, with g and u in memory between them).
+// Backward, from dh and the forward's g and u:
+//   dg = dh * u * act'(g),  du = dh * act(g)        rounded to the inputs' type (tensor-core operands)
+//   dx = dg . Wg + du . Wu,  dWg = dg^T . x,  dWu = du^T . x
+//
+// Forward (gated_fwd_kernel): both products of a tile share one accumulator: its columns
+// [0, FT) are gate features, [128, 128 + FT) the same features of up, so a thread finds both
+// values of a feature in its own TMEM lane and the epilogue forms h in registers; g and u never
+// leave the SM unless the backward needs them. On CTA pairs (N > 128: 256 tokens x 128
+// features) the pair UMMA takes half of its B rows from each CTA: the leader stages the gate
+// rows, its peer the up rows. Up to 128 tokens one CTA takes 128 tokens x 64 features with one
+// UMMA per projection, so that twice as many CTAs stream the weights, which is all that counts
+// there. Stages, loads (one 256-byte-row box per operand) and roles are those of the head's
+// kernels (lmce_engine.cuh, lmce_bwd_pair.cuh).
+//
+// With training the epilogue also keeps g and u in fp32, in blocks of 32 tokens x 32 features
+// laid out as the accumulator is read ([g | u][8 column groups of 4][32 tokens][4]), so each
+// store instruction of a warp writes 512 contiguous bytes. fp32 because dg and du are rounded
+// once already: with 16-bit g and u the gradients' error grew from 1.4 to 1.8 times that of a
+// single rounding, and the bytes are those an eager block keeps for its backward (g, u, act(g)
+// and h at 2 bytes each).
+//
+// e4m3 operands (serving): the same kernel with kind::f8f6f4, K = 256 per stage in the same
+// bytes; g and u are scaled by the row's and the feature's scale in the epilogue.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "lmce_bwd_pair.cuh"
+
+namespace lmce {
+
+constexpr int GT_GROUP = 8;        // row blocks that share a sweep over the column blocks
+constexpr int GATED_SAVE_BLOCK = 32 * 32;
+
+enum : int { ACT_SILU = 0, ACT_GELU_TANH = 1 };
+
+struct GatedParams {
+  int N, H, F;
+  int act;
+  float* saved;          // SAVE: blocks of 2 x 1024 fp32
+  const float* x_scale;  // e4m3: [N]
+  const float* g_scale;  // e4m3: [F]
+  const float* u_scale;
+  int* err;
+  unsigned long long timeout_ns;
+};
+
+// ------------------------------------------------------------- activation ---
+
+// sig = 1 / (1 + e), e = exp(-v), and v.
+__device__ __forceinline__ float act_sigmoid(float g, int act, float& e) {
+  const float v = act == ACT_SILU ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+  e = ex2_approx(-v * LOG2E);
+  return __fdividef(1.0f, 1.0f + e);
+}
+
+__device__ __forceinline__ float act_value(float g, int act) {
+  float e;
+  return g * act_sigmoid(g, act, e);
+}
+
+// act(g) and act'(g) = sig + g sig (1 - sig) v'
+__device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
+  float e;
+  const float s = act_sigmoid(g, act, e);
+  const float om = e < 1e30f ? e * s : 1.0f;  // 1 - sig, without its cancellation
+  const float dv = act == ACT_SILU ? 1.0f : 1.5957691216057308f * fmaf(0.134145f * g, g, 1.0f);
+  a = g * s;
+  da = fmaf(a * om, dv, s);
+}
+
+// ------------------------------------------------------------ tile orders ---
+
+// Row blocks in groups of GT_GROUP, column blocks across, row blocks of the group fastest: the
+// CTAs at work at one time cover a patch of the output that is about square, so each operand
+// panel that L2 holds serves several of them.
+__device__ __forceinline__ void grouped_tile(int u, int num_m, int num_n, int& m, int& n) {
+  const int per = GT_GROUP * num_n;
+  const int grp = u / per, m0 = grp * GT_GROUP;
+  const int gm = min(GT_GROUP, num_m - m0);
+  const int r = u - grp * per;
+  n = r / gm;
+  m = m0 + (r - n * gm);
+}
+
+template <bool PAIR>
+struct GatedCfg {
+  static constexpr int TOK = PAIR ? 256 : 128;  // tokens per tile
+  static constexpr int FT = PAIR ? 128 : 64;    // features per tile
+};
+
+// ---------------------------------------------------------------- forward ---
+
+template <bool E4M3, bool PAIR>
+__device__ __forceinline__ void gated_umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (PAIR && E4M3)
+    umma_f8_ss_pair(d, a, b, idesc, acc);
+  else if constexpr (PAIR)
+    umma_f16_ss_pair(d, a, b, idesc, acc);
+  else if constexpr (E4M3)
+    umma_f8_ss(d, a, b, idesc, acc);
+  else
+    umma_f16_ss(d, a, b, idesc, acc);
+}
+
+// BF16: the type of 16-bit operands and of h. The stage rows are 256 bytes whatever the type.
+template <bool BF16, bool E4M3, bool PAIR, bool SAVE>
+__global__ void __launch_bounds__(P_THREADS, 1)
+    gated_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
+                     const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_h,
+                     const GatedParams p) {
+  using C = GatedCfg<PAIR>;
+  constexpr int KB = E4M3 ? 2 * P_KB : P_KB;  // K per stage
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + P_STAGES * P_STAGE_BYTES);
+  uint64_t* empty_bar = full_bar + P_STAGES;
+  uint64_t* tfull_bar = empty_bar + P_STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0u;
+  const int unit0 = PAIR ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
+  const int step = PAIR ? static_cast<int>(cluster_count_x()) : static_cast<int>(gridDim.x);
+  const int num_m = (p.N + C::TOK - 1) / C::TOK, num_n = (p.F + C::FT - 1) / C::FT;
+  const int total = num_m * num_n;
+  const int nkb = (p.H + KB - 1) / KB;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], (PAIR ? 2 : 1) * P_EPI);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_g);
+    tma_prefetch_desc(&map_u);
+    tma_prefetch_desc(&map_h);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_holder, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_holder, TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const uint64_t tlimit = p.timeout_ns;
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer ---
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full_leader = PAIR ? mapa_shared(smem_u32(full_bar), 0) : 0u;
+      const CUtensorMap* map_b = rank == 0 ? &map_g : &map_u;
+      for (int u = unit0; ok && u < total; u += step) {
+        int m, n;
+        grouped_tile(u, num_m, num_n, m, n);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, tlimit)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + stage * P_STAGE_BYTES;
+          uint8_t* sb = sa + P_A_BYTES;
+          if constexpr (PAIR) {
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * P_STAGE_BYTES);
+            const uint32_t fb = full_leader + 8u * stage;
+            tma_load_3d_pair(sa, &map_x, fb, 0, m * C::TOK + BM * static_cast<int>(rank), 2 * kb);
+            tma_load_3d_pair(sb, map_b, fb, 0, n * C::FT, 2 * kb);
+          } else {
+            mbar_arrive_expect_tx(&full_bar[stage], P_STAGE_BYTES);
+            tma_load_3d(sa, &map_x, &full_bar[stage], 0, m * C::TOK, 2 * kb);
+            tma_load_3d(sb, &map_g, &full_bar[stage], 0, n * C::FT, 2 * kb);
+            tma_load_3d(sb + P_B_BYTES / 2, &map_u, &full_bar[stage], 0, n * C::FT, 2 * kb);
+          }
+          ++issued;
+          if (++stage == P_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+        if (rank == 0) {
+          const int outstanding = issued < P_STAGES ? issued : P_STAGES;
+          for (int i = 1; i <= outstanding; ++i) {
+            int s = stage - i;
+            uint32_t ph = phase;
+            if (s < 0) {
+              s += P_STAGES;
+              ph ^= 1u;
+            }
+            volatile int no_abort = 0;
+            mbar_wait(&full_bar[s], ph, &no_abort, tlimit);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- UMMA issuer ---
+    if (lane == 0 && rank == 0) {
+      // kind::f8f6f4's e4m3 has the format code that kind::f16 gives to f16
+      constexpr uint32_t idesc =
+          make_idesc_f16(BF16 && !E4M3, false, false, PAIR ? 2 * BM : BM, PAIR ? 2 * C::FT : C::FT);
+      const uint32_t peer_empty = PAIR ? mapa_shared(smem_u32(empty_bar), 1) : 0u;
+      const uint32_t peer_tfull = PAIR ? mapa_shared(smem_u32(tfull_bar), 1) : 0u;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int u = unit0; ok && u < total; u += step) {
+        if (!mbar_wait_cluster(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, tlimit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag, tlimit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * P_STAGE_BYTES);
+          const uint32_t sb = sa + P_A_BYTES;
+          // eight K steps of 32 bytes
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t accumulate = (kb | k) != 0 ? 1u : 0u;
+            if constexpr (PAIR) {
+              gated_umma<E4M3, true>(d_tmem, pair_operand_desc(sa, false, k), pair_operand_desc(sb, false, k), idesc,
+                                     accumulate);
+            } else {
+              // B: 64 rows per projection, their two 128-byte column blocks 8 KB apart
+              const uint32_t off = (k >> 2) * (BLOCK128_BYTES / 2) + (k & 3) * (UMMA_K * 2);
+              const uint64_t a = pair_operand_desc(sa, false, k);
+              gated_umma<E4M3, false>(d_tmem, a, smem_desc_sw128(sb + off, 16, 1024), idesc, accumulate);
+              gated_umma<E4M3, false>(d_tmem + 128, a, smem_desc_sw128(sb + P_B_BYTES / 2 + off, 16, 1024), idesc,
+                                      accumulate);
+            }
+          }
+          if constexpr (PAIR) {
+            umma_commit_pair(smem_u32(&empty_bar[stage]));
+            umma_commit_pair(peer_empty + 8u * stage);
+          } else {
+            umma_commit(&empty_bar[stage]);
+          }
+          if (++stage == P_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) {
+          umma_commit_pair(smem_u32(&tfull_bar[acc]));
+          umma_commit_pair(peer_tfull + 8u * acc);
+        } else {
+          umma_commit(&tfull_bar[acc]);
+        }
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+      }
+      if constexpr (PAIR)
+        umma_commit_pair(smem_u32(drain_bar));
+      else
+        umma_commit(drain_bar);
+      volatile int no_abort = 0;
+      mbar_wait(drain_bar, 0, &no_abort, tlimit);
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue ---
+    const int q = warp & 3;          // TMEM lane quadrant
+    const int ch = (warp - 2) >> 2;  // half of the tile's features this warp handles
+    uint8_t* xstage = smem + P_STAGES * P_STAGE_BYTES + 1024 + (warp - 2) * P_SLICE_BYTES;
+    const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t leader_tempty = PAIR ? mapa_shared(smem_u32(tempty_bar), 0) : 0u;
+    const int fblocks = p.F / 32;
+    int acc = 0, half = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int u = unit0; u < total; u += step) {
+      int m, n;
+      grouped_tile(u, num_m, num_n, m, n);
+      const int row0 = m * C::TOK + BM * static_cast<int>(rank) + q * 32;  // this warp's first token
+      float xs = 0.f;
+      if constexpr (E4M3) xs = row0 + lane < p.N ? p.x_scale[row0 + lane] : 0.f;
+      if (!mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, tlimit)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + lane_base + static_cast<uint32_t>(acc * BN);
+#pragma unroll 1
+      for (int c = ch * (C::FT / 64); c < (ch + 1) * (C::FT / 64); ++c) {
+        const int f0 = n * C::FT + c * 32;
+        uint32_t rg[32], ru[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + c * 32, rg);
+        tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
+        tmem_ld_wait(rg);
+        tmem_ld_wait(ru);
+        if (f0 >= p.F || row0 >= p.N) continue;  // F is a multiple of 64: a chunk lies wholly inside or past it
+        if constexpr (E4M3) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p.g_scale + f0) + j);
+            const float4 b = __ldg(reinterpret_cast<const float4*>(p.u_scale + f0) + j);
+            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              rg[4 * j + i] = __float_as_uint(__uint_as_float(rg[4 * j + i]) * xs * av[i]);
+              ru[4 * j + i] = __float_as_uint(__uint_as_float(ru[4 * j + i]) * xs * bv[i]);
+            }
+          }
+        }
+        if constexpr (SAVE) {
+          uint4* sv = reinterpret_cast<uint4*>(p.saved) +
+                      (static_cast<size_t>(row0 / 32) * fblocks + f0 / 32) * (2 * GATED_SAVE_BLOCK / 4) + lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sv[j * 32] = make_uint4(rg[4 * j], rg[4 * j + 1], rg[4 * j + 2], rg[4 * j + 3]);
+            sv[256 + j * 32] = make_uint4(ru[4 * j], ru[4 * j + 1], ru[4 * j + 2], ru[4 * j + 3]);
+          }
+        }
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = act_value(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
+        // one TMA store of the warp's 32 tokens x 32 features, through two 2 KB halves of its
+        // slice in turn (64-byte swizzle); tokens past N are clipped
+        uint8_t* box = xstage + half * 2048;
+        half ^= 1;
+        if (lane == 0) bulk_wait_read_1();
+        __syncwarp();
+        uint4* row = reinterpret_cast<uint4*>(box + lane * 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          row[i ^ ((lane >> 1) & 3)] =
+              make_uint4(pack2<BF16>(v[8 * i], v[8 * i + 1]), pack2<BF16>(v[8 * i + 2], v[8 * i + 3]),
+                         pack2<BF16>(v[8 * i + 4], v[8 * i + 5]), pack2<BF16>(v[8 * i + 6], v[8 * i + 7]));
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&map_h, box, f0, row0);
+          bulk_commit_group();
+        }
+      }
+      tc_fence_before();
+      if constexpr (PAIR)
+        mbar_arrive_cluster(leader_tempty + 8u * acc);
+      else
+        mbar_arrive(&tempty_bar[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    if (!ok) {
+      raise_error(p.err, ERR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else
+      tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// --------------------------------------------------- backward: dg and du ---
+
+// One warp per 32 tokens x 32 features of the saved blocks: g and u arrive as they were stored
+// (512 contiguous bytes per load), dh and the results pass through an 80-byte-pitch row staging
+// (conflict-free for 16-byte accesses by row and by column group). Memory-bound: 14 bytes per
+// element.
+constexpr int GATED_DACT_WARPS = 4;
+template <bool BF16>
+__global__ void __launch_bounds__(32 * GATED_DACT_WARPS)
+    gated_dact_kernel(const float4* __restrict__ saved, const uint4* __restrict__ dh, int n, int f, int act,
+                      uint4* __restrict__ dg, uint4* __restrict__ du) {
+  __shared__ uint4 st[GATED_DACT_WARPS][32][5];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int fb = f / 32, vec = f / 8;
+  const long long blocks = static_cast<long long>((n + 31) / 32) * fb;
+  for (long long b = static_cast<long long>(blockIdx.x) * GATED_DACT_WARPS + warp; b < blocks;
+       b += static_cast<long long>(gridDim.x) * GATED_DACT_WARPS) {
+    const int rb = static_cast<int>(b / fb), cb = static_cast<int>(b - static_cast<long long>(rb) * fb);
+    const float4* sv = saved + b * (2 * GATED_SAVE_BLOCK / 4) + lane;
+    float4 g[8], u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = __ldcs(sv + j * 32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = __ldcs(sv + 256 + j * 32);
+    const int c = lane & 3;
+    __syncwarp();  // the last block's rows have left the staging
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      const long long row = static_cast<long long>(rb) * 32 + r;
+      st[warp][r][c] = row < n ? __ldcs(dh + row * vec + cb * 4 + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncwarp();
+    float d[32];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack8<BF16>(st[warp][lane][i], d + 8 * i);
+    const float* gf = reinterpret_cast<const float*>(g);
+    const float* uf = reinterpret_cast<const float*>(u);
+    float e[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float a, da;
+      act_both(gf[j], act, a, da);
+      e[j] = d[j] * a;
+      d[j] = d[j] * uf[j] * da;
+    }
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st[warp][lane][i] = pack8<BF16>((pass ? e : d) + 8 * i);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const long long row = static_cast<long long>(rb) * 32 + r;
+        if (row < n) (pass ? du : dg)[row * vec + cb * 4 + c] = st[warp][r][c];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------ backward: the products ---
+
+// One launch for dx, dWg and dWu on CTA pairs. A unit is a 256 x 256 output tile with a range
+// of K stages:
+//   DX  256 tokens x 256 hidden, K over the gate features and then the up features (A = dg or
+//       du, K-major; B = the weight, MN-major); `splits` units share a tile when there are few
+//       tiles, each leaving an fp32 partial that gated_dx_sum_kernel adds in order
+//   DW  256 features x 256 hidden of one weight, K over the tokens (both operands MN-major)
+// DX units are the longer ones and come first; the pairs that get one DX unit less than the
+// others take that many stages' worth of DW units before the rest is dealt out in turn. The
+// assignment is a function of the sizes alone: no counters, the same sums every time.
+struct GatedBwdParams {
+  int N, H, F;
+  int n_dx, splits, dx_stages;   // DX units (tiles x splits), splits per tile, K stages of a whole tile
+  int n_dw, dw_first;            // DW units; first weight wanted (0 gate, 1 up)
+  int rows_pad;                  // rows of one split's partial
+  int* err;
+  unsigned long long timeout_ns;
+};
+
+struct GatedUnits {
+  int pair, pairs, n_dx, n_dw;
+  int extra, extra_step, extra_at;   // DW units this pair takes ahead of the rest
+  int common;                        // first DW unit of the common part
+  int phase, next;
+
+  __device__ __forceinline__ void init(const GatedBwdParams& p, int pair_, int pairs_) {
+    pair = pair_;
+    pairs = pairs_;
+    n_dx = p.n_dx;
+    n_dw = p.n_dw;
+    const int heavy = n_dx % pairs;
+    const int light = heavy ? pairs - heavy : 0;
+    const int lx = p.splits > 0 ? p.dx_stages / p.splits : 0;
+    const int ld = max(1, (p.N + P_KB - 1) / P_KB);
+    const int ahead = light ? lx / ld : 0;
+    common = static_cast<int>(min(static_cast<long long>(n_dw), static_cast<long long>(light) * ahead));
+    extra = pair >= heavy && light ? ahead : 0;
+    extra_step = light;
+    extra_at = pair - heavy;
+    phase = 0;
+    next = pair;
+  }
+
+  // The next unit: a DX unit's index, or n_dx + a DW unit's index; -1 at the end.
+  __device__ __forceinline__ int get() {
+    if (phase == 0) {
+      if (next < n_dx) {
+        const int u = next;
+        next += pairs;
+        return u;
+      }
+      phase = 1;
+    }
+    if (phase == 1) {
+      if (extra > 0 && extra_at < common) {
+        const int u = extra_at;
+        extra_at += extra_step;
+        --extra;
+        return n_dx + u;
+      }
+      phase = 2;
+      next = common + pair;
+    }
+    if (next >= n_dw) return -1;
+    const int u = next;
+    next += pairs;
+    return n_dx + u;
+  }
+};
+
+struct GatedTile {
+  bool dx;
+  int which;        // DW: 0 gate, 1 up
+  int m, n;         // row block, column block
+  int split;
+  int k0, k1;       // stages
+
+  __device__ __forceinline__ void decode(const GatedBwdParams& p, int u) {
+    const int nh = (p.H + 255) / 256;
+    dx = u < p.n_dx;
+    which = 0;
+    split = 0;
+    k0 = 0;
+    if (dx) {
+      const int tiles = p.n_dx / p.splits;
+      split = u / tiles;
+      grouped_tile(u - split * tiles, (p.N + 255) / 256, nh, m, n);
+      k0 = static_cast<int>(static_cast<long long>(split) * p.dx_stages / p.splits);
+      k1 = static_cast<int>(static_cast<long long>(split + 1) * p.dx_stages / p.splits);
+    } else {
+      const int per = nh * ((p.F + 255) / 256);
+      int i = u - p.n_dx;
+      which = p.dw_first + i / per;
+      i %= per;
+      m = i / nh;
+      n = i - m * nh;
+      k1 = (p.N + P_KB - 1) / P_KB;
+    }
+  }
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(P_THREADS, 1)
+    gated_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_wg,
+                     const __grid_constant__ CUtensorMap map_wu, const __grid_constant__ CUtensorMap map_dg,
+                     const __grid_constant__ CUtensorMap map_du, const __grid_constant__ CUtensorMap map_dx,
+                     const __grid_constant__ CUtensorMap map_dwg, const __grid_constant__ CUtensorMap map_dwu,
+                     const GatedBwdParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + P_STAGES * P_STAGE_BYTES);
+  uint64_t* empty_bar = full_bar + P_STAGES;
+  uint64_t* tfull_bar = empty_bar + P_STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(cluster_count_x());
+  const int fstages = (p.F + P_KB - 1) / P_KB;  // stages of one weight's features
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], 2 * P_EPI);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_holder, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const uint64_t tlimit = p.timeout_ns;
+  GatedUnits units;
+  units.init(p, pair, pairs);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
+      const int r = static_cast<int>(rank);
+      for (int u = units.get(); ok && u >= 0; u = units.get()) {
+        GatedTile t;
+        t.decode(p, u);
+        const CUtensorMap* dw_a = t.which ? &map_du : &map_dg;
+        for (int kb = t.k0; kb < t.k1; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, tlimit)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + stage * P_STAGE_BYTES;
+          uint8_t* sb = sa + P_A_BYTES;
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * P_STAGE_BYTES);
+          const uint32_t fb = full_leader + 8u * stage;
+          const int nblk = (t.n * 256 + BM * r) / 64;
+          if (t.dx) {
+            const bool up = kb >= fstages;
+            const int k = up ? kb - fstages : kb;
+            tma_load_3d_pair(sa, up ? &map_du : &map_dg, fb, 0, t.m * 256 + BM * r, 2 * k);
+            tma_load_3d_pair(sb, up ? &map_wu : &map_wg, fb, 0, k * P_KB, nblk);
+          } else {
+            tma_load_3d_pair(sa, dw_a, fb, 0, kb * P_KB, (t.m * 256 + BM * r) / 64);
+            tma_load_3d_pair(sb, &map_x, fb, 0, kb * P_KB, nblk);
+          }
+          ++issued;
+          if (++stage == P_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+        if (rank == 0) {
+          const int outstanding = issued < P_STAGES ? issued : P_STAGES;
+          for (int i = 1; i <= outstanding; ++i) {
+            int s = stage - i;
+            uint32_t ph = phase;
+            if (s < 0) {
+              s += P_STAGES;
+              ph ^= 1u;
+            }
+            volatile int no_abort = 0;
+            mbar_wait(&full_bar[s], ph, &no_abort, tlimit);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
+      const uint32_t peer_tfull = mapa_shared(smem_u32(tfull_bar), 1);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      long long waited = 0;
+      for (int u = units.get(); u >= 0; u = units.get()) {
+        GatedTile t;
+        t.decode(p, u);
+        if (!mbar_wait_cluster(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, tlimit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        ok = t.dx ? mma_tile_pair<BF16, false, true, BN>(smem, full_bar, empty_bar, peer_empty, t.k1 - t.k0, d_tmem,
+                                                         stage, phase, abort_flag, tlimit, waited)
+                  : mma_tile_pair<BF16, true, true, BN>(smem, full_bar, empty_bar, peer_empty, t.k1 - t.k0, d_tmem,
+                                                        stage, phase, abort_flag, tlimit, waited);
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&tfull_bar[acc]));
+        umma_commit_pair(peer_tfull + 8u * acc);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+      }
+      umma_commit_pair(smem_u32(drain_bar));
+      volatile int no_abort = 0;
+      mbar_wait(drain_bar, 0, &no_abort, tlimit);
+    }
+  } else {
+    const int q = warp & 3;
+    const int ch = (warp - 2) >> 2;
+    uint8_t* xstage = smem + P_STAGES * P_STAGE_BYTES + 1024 + (warp - 2) * P_SLICE_BYTES;
+    const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t leader_tempty = mapa_shared(smem_u32(tempty_bar), 0);
+    int acc = 0, half = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int u = units.get(); u >= 0; u = units.get()) {
+      GatedTile t;
+      t.decode(p, u);
+      const int row0 = t.m * 256 + BM * static_cast<int>(rank) + q * 32;
+      const int rows = t.dx ? p.N : p.F;
+      const CUtensorMap* map_o = t.dx ? &map_dx : t.which ? &map_dwu : &map_dwg;
+      const bool partial = t.dx && p.splits > 1;
+      if (!mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, tlimit)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + lane_base + static_cast<uint32_t>(acc * BN);
+#pragma unroll 1
+      for (int c = ch * 4; c < ch * 4 + 4; ++c) {
+        const int h0 = t.n * 256 + c * 32;
+        uint32_t raw[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + c * 32, raw);
+        tmem_ld_wait(raw);
+        if (h0 >= p.H || row0 >= rows) continue;  // H is a multiple of 64
+        if (partial) {
+          // 32 x 32 fp32 in the 128-byte swizzled box layout, the whole slice
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          uint4* sl = reinterpret_cast<uint4*>(xstage);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            sl[lane * 8 + (i ^ (lane & 7))] =
+                make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map_o, xstage, h0, t.split * p.rows_pad + row0);
+            bulk_commit_group();
+          }
+          half = 0;
+        } else {
+          uint8_t* box = xstage + half * 2048;
+          half ^= 1;
+          if (lane == 0) bulk_wait_read_1();  // the box of two stores ago has left it
+          __syncwarp();
+          uint4* row = reinterpret_cast<uint4*>(box + lane * 64);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            row[i ^ ((lane >> 1) & 3)] = make_uint4(
+                pack2<BF16>(__uint_as_float(raw[8 * i]), __uint_as_float(raw[8 * i + 1])),
+                pack2<BF16>(__uint_as_float(raw[8 * i + 2]), __uint_as_float(raw[8 * i + 3])),
+                pack2<BF16>(__uint_as_float(raw[8 * i + 4]), __uint_as_float(raw[8 * i + 5])),
+                pack2<BF16>(__uint_as_float(raw[8 * i + 6]), __uint_as_float(raw[8 * i + 7])));
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map_o, box, h0, row0);
+            bulk_commit_group();
+          }
+        }
+      }
+      if (partial && lane == 0) bulk_wait_read_all();  // the next unit may use the slice as two boxes
+      tc_fence_before();
+      mbar_arrive_cluster(leader_tempty + 8u * acc);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    if (!ok) {
+      raise_error(p.err, ERR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// dx = dtype(sum over splits of the fp32 partials, in order); rows of `vec` 4-value units.
+template <bool BF16>
+__global__ void gated_dx_sum_kernel(const float4* __restrict__ part, int splits, long long split_stride,
+                                    long long total, uint2* __restrict__ dx) {
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    float4 v = __ldcs(part + i);
+    for (int s = 1; s < splits; ++s) {
+      const float4 w = __ldcs(part + s * split_stride + i);
+      v.x += w.x;
+      v.y += w.y;
+      v.z += w.z;
+      v.w += w.w;
+    }
+    dx[i] = make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
+  }
+}
+
+}  // namespace lmce

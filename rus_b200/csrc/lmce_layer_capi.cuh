@@ -1,4 +1,5 @@
-// C entries of the operators around the head: residual add + RMSNorm and gradient clipping.
+// C entries of the operators around the head: residual add + RMSNorm, the gated projection of a
+// feed-forward block, and gradient clipping.
 // Part of lmce_capi.cu (it uses that file's error, device and launch helpers).
 #pragma once
 
@@ -6,6 +7,7 @@
 #include <new>
 
 #include "lmce_addnorm.cuh"
+#include "lmce_gated.cuh"
 #include "lmce_gradnorm.cuh"
 
 namespace {
@@ -15,7 +17,7 @@ namespace {
 constexpr int kAnThreads = 512;      // most threads of a row
 constexpr int kAnBlock = 256;        // threads a block is filled up to with rows
 constexpr int kAnBwdBlocks = 592;    // partial rows of dw: four blocks on each of 148 SMs
-constexpr int64_t kAnMaxHidden = 32768;
+constexpr int64_t kAnMaxHidden = 16384;
 
 struct RowShape {
   int vpt, threads, rows;
@@ -23,7 +25,7 @@ struct RowShape {
 
 // Threads and vectors per thread for a row of `vec` 16-byte vectors: one vector per thread
 // while rows are few (latency), two when there are enough rows to fill the SMs (more loads in
-// flight per thread), more where a row would need over 512 threads.
+// flight per thread), four where a row would need over 512 threads.
 RowShape row_shape(int64_t n, int vec, int sms) {
   RowShape s;
   s.vpt = n > 4ll * sms && vec > 32 ? 2 : 1;
@@ -40,8 +42,7 @@ void launch_add_norm(const AddNormParams& p, int vpt, int grid, cudaStream_t st)
   switch (vpt) {
     case 1: add_norm_kernel<BF16, 1, E4M3><<<grid, threads, 0, st>>>(p); break;
     case 2: add_norm_kernel<BF16, 2, E4M3><<<grid, threads, 0, st>>>(p); break;
-    case 4: add_norm_kernel<BF16, 4, E4M3><<<grid, threads, 0, st>>>(p); break;
-    default: add_norm_kernel<BF16, 8, E4M3><<<grid, threads, 0, st>>>(p); break;
+    default: add_norm_kernel<BF16, 4, E4M3><<<grid, threads, 0, st>>>(p); break;
   }
 }
 
@@ -51,8 +52,7 @@ void launch_add_norm_bwd(const AddNormBwdParams& p, int vpt, int grid, size_t sm
   switch (vpt) {
     case 1: add_norm_bwd_kernel<BF16, 1><<<grid, threads, smem, st>>>(p); break;
     case 2: add_norm_bwd_kernel<BF16, 2><<<grid, threads, smem, st>>>(p); break;
-    case 4: add_norm_bwd_kernel<BF16, 4><<<grid, threads, smem, st>>>(p); break;
-    default: add_norm_bwd_kernel<BF16, 8><<<grid, threads, smem, st>>>(p); break;
+    default: add_norm_bwd_kernel<BF16, 4><<<grid, threads, smem, st>>>(p); break;
   }
 }
 
@@ -136,6 +136,107 @@ int launch_clip(bool scale, void* const* grads, const int64_t* numels, const int
     grad_norm_kernel<MAXT><<<kGnBlocks, GN_THREADS, 0, st>>>(b, partial);
   }
   return launched();
+}
+
+// ------------------------------------------------------- gated projection ---
+
+constexpr int64_t kGatedMaxRows = 1ll << 26;   // tiles and token indices stay within 32 bits
+constexpr int64_t kGatedMaxDim = 1ll << 20;
+constexpr int kGatedPairs = 74;                // CTA pairs the backward's K splits are sized for
+constexpr int kGatedMaxSplits = 16;
+
+// [outer][inner] bytes (e4m3) as a 3-D view {128, outer, inner / 128 blocks}, 128-byte swizzle:
+// the boxes hold the same bytes as those of 64 16-bit values (make_map_3d).
+int make_map_3d_bytes(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint32_t box_y,
+                      uint32_t box_z) {
+  cuuint64_t dims[3] = {128, outer, inner / 128};
+  cuuint64_t strides[2] = {inner, 128};
+  cuuint32_t box[3] = {128, box_y, box_z};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LMCE_ERR_CUDA, "cuTensorMapEncodeTiled (bytes) failed (%d)", static_cast<int>(r));
+  return LMCE_OK;
+}
+
+template <bool BF16, bool E4M3, bool PAIR, bool SAVE>
+int launch_gated(const CUtensorMap* maps, const GatedParams& p, int sms, cudaStream_t st) {
+  using C = GatedCfg<PAIR>;
+  auto kern = gated_fwd_kernel<BF16, E4M3, PAIR, SAVE>;
+  static bool done[kMaxDevices] = {};
+  if (int rc = ensure_smem_attr(kern, PBWD_SMEM_BYTES, done)) return rc;
+  static int cache[kMaxDevices] = {};
+  const int slots = PAIR ? max_pairs(kern, PBWD_SMEM_BYTES, sms, cache, P_THREADS) : sms;
+  const int64_t units = static_cast<int64_t>((p.N + C::TOK - 1) / C::TOK) * ((p.F + C::FT - 1) / C::FT);
+  const int grid = static_cast<int>(std::min<int64_t>(units, slots)) * (PAIR ? 2 : 1);
+  return launch_ex(kern, grid, P_THREADS, PBWD_SMEM_BYTES, PAIR ? 2 : 1, st, maps[0], maps[1], maps[2], maps[3], p);
+}
+
+template <bool BF16, bool E4M3>
+int launch_gated_any(const CUtensorMap* maps, const GatedParams& p, bool pair, int sms, cudaStream_t st) {
+  if constexpr (!E4M3) {
+    if (p.saved != nullptr)
+      return pair ? launch_gated<BF16, E4M3, true, true>(maps, p, sms, st)
+                  : launch_gated<BF16, E4M3, false, true>(maps, p, sms, st);
+  }
+  return pair ? launch_gated<BF16, E4M3, true, false>(maps, p, sms, st)
+              : launch_gated<BF16, E4M3, false, false>(maps, p, sms, st);
+}
+
+int check_gated(int64_t n, int64_t h, int64_t f, int dtype, int act, int64_t h_step) {
+  if (n <= 0 || n > kGatedMaxRows) return fail(LMCE_ERR_INVALID_ARGUMENT, "bad n_rows");
+  if (h <= 0 || h % h_step != 0 || h > kGatedMaxDim)
+    return fail(LMCE_ERR_UNSUPPORTED, "hidden_dim must be a multiple of %lld", (long long)h_step);
+  if (f <= 0 || f % 64 != 0 || f > kGatedMaxDim) return fail(LMCE_ERR_UNSUPPORTED, "ffn_dim must be a multiple of 64");
+  if (((n + 127) / 128) * ((f + 63) / 64) > 0x7fffffffll || ((n + 255) / 256) * ((h + 255) / 256) > 0x3ffffffll)
+    return fail(LMCE_ERR_UNSUPPORTED, "too many tiles");
+  if (dtype != LMCE_DTYPE_F16 && dtype != LMCE_DTYPE_BF16) return fail(LMCE_ERR_UNSUPPORTED, "dtype %d", dtype);
+  if (act != LMCE_ACT_SILU && act != LMCE_ACT_GELU_TANH) return fail(LMCE_ERR_UNSUPPORTED, "activation %d", act);
+  return LMCE_OK;
+}
+
+struct GatedBwdLayout {
+  size_t dg, du, part, total;
+  int splits, stages, rows_pad;
+};
+
+// K splits of a dx tile: enough that no unit is longer than about half of what a pair gets
+// of the whole work, so that a few tiles with a long K (few tokens) do not hold up the rest
+// (693 x 1536 x 8960: 18 tiles of 140 stages next to 420 dW units of 6, 68 stages per pair).
+GatedBwdLayout gated_bwd_layout(int64_t n, int64_t h, int64_t f, bool want_dx, int n_weights) {
+  GatedBwdLayout L = {};
+  const int64_t tiles = ((n + 255) / 256) * ((h + 255) / 256);
+  const int64_t dw = n_weights * ((f + 255) / 256) * ((h + 255) / 256) * ((n + 127) / 128);
+  L.stages = static_cast<int>(2 * ((f + 127) / 128));
+  L.splits = 1;
+  if (want_dx) {
+    const int64_t share = std::max<int64_t>(1, (tiles * L.stages + dw) / kGatedPairs);
+    L.splits = static_cast<int>(std::min<int64_t>({(2 * L.stages + share - 1) / share, kGatedMaxSplits, L.stages}));
+    if (L.splits < 1 || 2 * share >= 3 * L.stages) L.splits = 1;
+  }
+  L.rows_pad = static_cast<int>((n + 255) / 256 * 256);
+  size_t off = 0;
+  L.dg = off;
+  off = align_up(off + static_cast<size_t>(n) * f * 2, 256);
+  L.du = off;
+  off = align_up(off + static_cast<size_t>(n) * f * 2, 256);
+  L.part = off;
+  if (want_dx && L.splits > 1) off = align_up(off + static_cast<size_t>(L.splits) * L.rows_pad * h * 4, 256);
+  L.total = off;
+  return L;
+}
+
+template <bool BF16>
+int launch_gated_bwd(const CUtensorMap* maps, const GatedBwdParams& p, int sms, cudaStream_t st) {
+  auto kern = gated_bwd_kernel<BF16>;
+  static bool done[kMaxDevices] = {};
+  if (int rc = ensure_smem_attr(kern, PBWD_SMEM_BYTES, done)) return rc;
+  static int cache[kMaxDevices] = {};
+  const int slots = max_pairs(kern, PBWD_SMEM_BYTES, sms, cache, P_THREADS);
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.n_dx) + p.n_dw, slots));
+  return launch_ex(kern, grid, P_THREADS, PBWD_SMEM_BYTES, 2, st, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5],
+                   maps[6], maps[7], p);
 }
 
 }  // namespace
@@ -264,6 +365,158 @@ int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t
     }
   }
   return LMCE_OK;
+}
+
+size_t lmce_gated_saved_bytes(int64_t n_rows, int64_t ffn_dim) {
+  if (n_rows <= 0 || ffn_dim <= 0) return 0;
+  return static_cast<size_t>((n_rows + 31) / 32 * 32) * ffn_dim * 8;
+}
+
+int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64_t n_rows, int64_t hidden_dim,
+                      int64_t ffn_dim, int dtype, int act, void* h_out, void* saved, void* stream) {
+  if (!x || !w_gate || !w_up || !h_out) return fail(LMCE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (int rc = check_gated(n_rows, hidden_dim, ffn_dim, dtype, act, 64)) return rc;
+  if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(h_out) || !aligned16(saved))
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "misaligned buffers");
+  DevInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  if (int rc = get_encoder()) return rc;
+  const bool bf16 = dtype == LMCE_DTYPE_BF16, pair = n_rows > BM;
+  const uint32_t w_rows = pair ? 128 : 64;
+  CUtensorMap maps[4];
+  if (int rc = make_map_3d(&maps[0], x, bf16, hidden_dim, n_rows, hidden_dim, 128, 2)) return rc;
+  if (int rc = make_map_3d(&maps[1], w_gate, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, 2)) return rc;
+  if (int rc = make_map_3d(&maps[2], w_up, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, 2)) return rc;
+  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
+  GatedParams p = {};
+  p.N = static_cast<int>(n_rows);
+  p.H = static_cast<int>(hidden_dim);
+  p.F = static_cast<int>(ffn_dim);
+  p.act = act;
+  p.saved = static_cast<float*>(saved);
+  p.err = d->err_ptr;
+  p.timeout_ns = wait_timeout_ns();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return bf16 ? launch_gated_any<true, false>(maps, p, pair, d->sms, st)
+              : launch_gated_any<false, false>(maps, p, pair, d->sms, st);
+}
+
+int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const void* w_gate, const float* gate_scale,
+                           const void* w_up, const float* up_scale, int64_t n_rows, int64_t hidden_dim,
+                           int64_t ffn_dim, int out_dtype, int act, void* h_out, void* stream) {
+  if (!x || !x_scale || !w_gate || !gate_scale || !w_up || !up_scale || !h_out)
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (int rc = check_gated(n_rows, hidden_dim, ffn_dim, out_dtype, act, 128)) return rc;
+  if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(h_out) || !aligned16(gate_scale) ||
+      !aligned16(up_scale) || reinterpret_cast<uintptr_t>(x_scale) % 4 != 0)
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "misaligned buffers");
+  DevInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  if (int rc = get_encoder()) return rc;
+  const bool bf16 = out_dtype == LMCE_DTYPE_BF16, pair = n_rows > BM;
+  const uint32_t w_rows = pair ? 128 : 64;
+  CUtensorMap maps[4];
+  if (int rc = make_map_3d_bytes(&maps[0], x, hidden_dim, n_rows, 128, 2)) return rc;
+  if (int rc = make_map_3d_bytes(&maps[1], w_gate, hidden_dim, ffn_dim, w_rows, 2)) return rc;
+  if (int rc = make_map_3d_bytes(&maps[2], w_up, hidden_dim, ffn_dim, w_rows, 2)) return rc;
+  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
+  GatedParams p = {};
+  p.N = static_cast<int>(n_rows);
+  p.H = static_cast<int>(hidden_dim);
+  p.F = static_cast<int>(ffn_dim);
+  p.act = act;
+  p.x_scale = x_scale;
+  p.g_scale = gate_scale;
+  p.u_scale = up_scale;
+  p.err = d->err_ptr;
+  p.timeout_ns = wait_timeout_ns();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return bf16 ? launch_gated_any<true, true>(maps, p, pair, d->sms, st)
+              : launch_gated_any<false, true>(maps, p, pair, d->sms, st);
+}
+
+size_t lmce_gated_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int want_dx,
+                                      int n_weights) {
+  if (n_rows <= 0 || hidden_dim <= 0 || ffn_dim <= 0) return 0;
+  return gated_bwd_layout(n_rows, hidden_dim, ffn_dim, want_dx != 0, n_weights).total;
+}
+
+int lmce_gated_backward(const void* d_h, const void* saved, const void* x, const void* w_gate, const void* w_up,
+                        int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int dtype, int act, void* d_x,
+                        void* d_gate, void* d_up, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!d_h || !saved || !x || !w_gate || !w_up || !workspace || (!d_x && !d_gate && !d_up))
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "null pointer");
+  if (int rc = check_gated(n_rows, hidden_dim, ffn_dim, dtype, act, 64)) return rc;
+  if (!aligned16(d_h) || !aligned16(saved) || !aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) ||
+      !aligned16(d_x) || !aligned16(d_gate) || !aligned16(d_up) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "misaligned buffers");
+  const int n_weights = (d_gate ? 1 : 0) + (d_up ? 1 : 0);
+  const GatedBwdLayout L = gated_bwd_layout(n_rows, hidden_dim, ffn_dim, d_x != nullptr, n_weights);
+  if (workspace_bytes < L.total) return fail(LMCE_ERR_WORKSPACE, "workspace too small");
+  DevInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  if (int rc = get_encoder()) return rc;
+  const bool bf16 = dtype == LMCE_DTYPE_BF16;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  void *dg = ws + L.dg, *du = ws + L.du;
+  float* part = reinterpret_cast<float*>(ws + L.part);
+  const int64_t n = n_rows, h = hidden_dim, f = ffn_dim;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  const int64_t blocks = (n + 31) / 32 * (f / 32);
+  const int dgrid = static_cast<int>(
+      std::min<int64_t>((blocks + GATED_DACT_WARPS - 1) / GATED_DACT_WARPS, d->sms * 16ll));
+  if (bf16)
+    gated_dact_kernel<true><<<dgrid, 32 * GATED_DACT_WARPS, 0, st>>>(
+        static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
+        act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
+  else
+    gated_dact_kernel<false><<<dgrid, 32 * GATED_DACT_WARPS, 0, st>>>(
+        static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
+        act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
+  if (int rc = launched()) return rc;
+
+  CUtensorMap maps[8];
+  if (int rc = make_map_3d(&maps[0], x, bf16, h, n, h, 128, 2)) return rc;
+  if (int rc = make_map_3d(&maps[1], w_gate, bf16, h, f, h, 128, 2)) return rc;
+  if (int rc = make_map_3d(&maps[2], w_up, bf16, h, f, h, 128, 2)) return rc;
+  if (int rc = make_map_3d(&maps[3], dg, bf16, f, n, f, 128, 2)) return rc;
+  if (int rc = make_map_3d(&maps[4], du, bf16, f, n, f, 128, 2)) return rc;
+  // outputs that are not wanted keep a valid map that no unit uses
+  if (d_x && L.splits > 1) {
+    if (int rc = make_map_f32(&maps[5], part, h, static_cast<uint64_t>(L.splits) * L.rows_pad, h, 32, 32)) return rc;
+  } else if (int rc = make_map_store16(&maps[5], d_x ? d_x : dg, bf16, d_x ? h : f, n, d_x ? h : f)) {
+    return rc;
+  }
+  if (int rc = make_map_store16(&maps[6], d_gate ? d_gate : dg, bf16, d_gate ? h : f, d_gate ? f : n, d_gate ? h : f))
+    return rc;
+  if (int rc = make_map_store16(&maps[7], d_up ? d_up : dg, bf16, d_up ? h : f, d_up ? f : n, d_up ? h : f)) return rc;
+
+  const int64_t nh = (h + 255) / 256;
+  GatedBwdParams p = {};
+  p.N = static_cast<int>(n);
+  p.H = static_cast<int>(h);
+  p.F = static_cast<int>(f);
+  p.splits = d_x ? L.splits : 1;
+  p.n_dx = d_x ? static_cast<int>((n + 255) / 256 * nh) * L.splits : 0;
+  p.dx_stages = L.stages;
+  p.n_dw = n_weights * static_cast<int>((f + 255) / 256 * nh);
+  p.dw_first = d_gate ? 0 : 1;
+  p.rows_pad = L.rows_pad;
+  p.err = d->err_ptr;
+  p.timeout_ns = wait_timeout_ns();
+  if (int rc = bf16 ? launch_gated_bwd<true>(maps, p, d->sms, st) : launch_gated_bwd<false>(maps, p, d->sms, st))
+    return rc;
+  if (!d_x || L.splits == 1) return LMCE_OK;
+  const long long total = n * h / 4, stride = static_cast<long long>(L.rows_pad) * h / 4;
+  const int sgrid = static_cast<int>(std::min<long long>((total + 255) / 256, d->sms * 8ll));
+  if (bf16)
+    gated_dx_sum_kernel<true><<<sgrid, 256, 0, st>>>(reinterpret_cast<const float4*>(part), L.splits, stride, total,
+                                                     static_cast<uint2*>(d_x));
+  else
+    gated_dx_sum_kernel<false><<<sgrid, 256, 0, st>>>(reinterpret_cast<const float4*>(part), L.splits, stride, total,
+                                                      static_cast<uint2*>(d_x));
+  return launched();
 }
 
 }  // extern "C"

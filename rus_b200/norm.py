@@ -34,9 +34,9 @@ def _check(x, residual, weight, who: str) -> None:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: residual must have the shape of x")
     if weight.device != x.device or (residual is not None and residual.device != x.device):
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: all tensors must be on the same device")
-    if x.shape[-1] % 8 != 0 or not 0 < x.shape[-1] <= 32768:
+    if x.shape[-1] % 8 != 0 or not 0 < x.shape[-1] <= 16384:
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
-                             f"{who}: hidden size {x.shape[-1]} (need a multiple of 8, at most 32768)")
+                             f"{who}: hidden size {x.shape[-1]} (need a multiple of 8, at most 16384)")
 
 
 def _forward(x, residual, weight, eps, keep_rstd: bool):
