@@ -10,6 +10,8 @@ import ctypes
 import threading
 from pathlib import Path
 
+import torch
+
 LIB_PATH = Path(__file__).resolve().parent / "liblmce.so"
 
 LMCE_OK = 0
@@ -162,6 +164,21 @@ def call(name: str, *args) -> int:
     rc = fn(*args)
     check(rc)
     return rc
+
+
+def launch(device, name: str, *args) -> None:
+    """Call ``name`` (whose last argument is the stream) on ``device``'s current stream, with
+    ``device`` current. The short way of small operators, whose time is the host's: no context
+    manager where the device is current already, and the stream's handle without its object."""
+    fn = getattr(_lib or load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != LMCE_OK:
+        check(rc)
 
 
 def launch_count() -> int:

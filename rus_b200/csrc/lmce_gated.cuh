@@ -13,9 +13,8 @@
 // values of a feature in its own TMEM lane and the epilogue forms h in registers; g and u never
 // leave the SM unless the backward needs them. On CTA pairs (N > 128: 256 tokens x 128
 // features) the pair UMMA takes half of its B rows from each CTA: the leader stages the gate
-// rows, its peer the up rows. Up to 128 tokens one CTA takes 128 tokens x 64 features with one
-// UMMA per projection, so that twice as many CTAs stream the weights, which is all that counts
-// there. Stages, loads (one 256-byte-row box per operand) and roles are those of the head's
+// rows, its peer the up rows. Up to 128 tokens (gated_few_kernel, gated_token_kernel) the weights'
+// read is all that counts. Stages, loads (one 256-byte-row box per operand) and roles are those of the head's
 // kernels (lmce_engine.cuh, lmce_bwd_pair.cuh).
 //
 // With training the epilogue also keeps g and u in fp32, in blocks of 32 tokens x 32 features
@@ -32,6 +31,7 @@
 #include <cuda_fp8.h>
 
 #include "lmce_bwd_pair.cuh"
+#include "lmce_rmsnorm.cuh"
 
 namespace lmce {
 
@@ -43,6 +43,7 @@ enum : int { ACT_SILU = 0, ACT_GELU_TANH = 1 };
 struct GatedParams {
   int N, H, F;
   int act;
+  int b_rows;            // up to 128 tokens: token rows per stage, N rounded up to 16
   float* saved;          // SAVE: blocks of 2 x 1024 fp32
   const float* x_scale;  // e4m3: [N]
   const float* g_scale;  // e4m3: [F]
@@ -75,6 +76,87 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) 
   da = fmaf(a * om, dv, s);
 }
 
+// ------------------------------------------------------------ few tokens ---
+
+// One token without a backward: one warp per feature reads its gate and its up row once, 16
+// bytes per lane, and multiplies both with the token in fp32 (the token, a few KB, comes from
+// L1). The weights' read is all that counts, and it has no pipeline to fill: 32 lanes x 2 x
+// GT_UNROLL loads of 16 bytes are in flight per warp from its first instruction on. One B200,
+// 16 bits: 1536 x 8960 10.5 us (floor 8.6, gated_few_kernel 13.2), 3584 x 18944 41.3 us (floor
+// 42.2, 43.9). A second token costs this kernel as many instructions again (14.1 and 48.4 us)
+// and the other one nothing, so it has one only.
+constexpr int GT_WARPS = 4;
+constexpr int GT_UNROLL = 4;
+
+template <bool BF16, bool E4M3>
+__device__ __forceinline__ void unpack_operand(const uint4& u, float* f) {
+  if constexpr (E4M3) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const __half2_raw hr =
+            __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w[i] >> (16 * k)) & 0xffffu), __NV_E4M3);
+        const float2 v = __half22float2(__half2(hr));
+        f[4 * i + 2 * k] = v.x;
+        f[4 * i + 2 * k + 1] = v.y;
+      }
+    }
+  } else {
+    unpack8<BF16>(u, f);
+  }
+}
+
+// vec: 16-byte units per row.
+template <bool BF16, bool E4M3>
+__global__ void __launch_bounds__(32 * GT_WARPS)
+    gated_token_kernel(const uint4* __restrict__ x, const uint4* __restrict__ wg, const uint4* __restrict__ wu,
+                       int vec, const GatedParams p, uint16_t* __restrict__ h) {
+  constexpr int PER = E4M3 ? 16 : 8;
+  const int lane = threadIdx.x & 31;
+  const int f = blockIdx.x * GT_WARPS + threadIdx.x / 32;
+  if (f >= p.F) return;
+  const uint4* rg = wg + static_cast<size_t>(f) * vec;
+  const uint4* ru = wu + static_cast<size_t>(f) * vec;
+  float g = 0.f, u = 0.f;
+  for (int c0 = lane; c0 < vec; c0 += 32 * GT_UNROLL) {
+    uint4 a[GT_UNROLL], b[GT_UNROLL];
+#pragma unroll
+    for (int i = 0; i < GT_UNROLL; ++i) {
+      const int c = c0 + 32 * i;
+      a[i] = b[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < vec) {
+        a[i] = __ldcs(rg + c);
+        b[i] = __ldcs(ru + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < GT_UNROLL; ++i) {
+      const int c = c0 + 32 * i;
+      if (c >= vec) break;
+      float fa[PER], fb[PER], fx[PER];
+      unpack_operand<BF16, E4M3>(a[i], fa);
+      unpack_operand<BF16, E4M3>(b[i], fb);
+      unpack_operand<BF16, E4M3>(__ldg(x + c), fx);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        g = fmaf(fx[j], fa[j], g);
+        u = fmaf(fx[j], fb[j], u);
+      }
+    }
+  }
+  g = warp_sum(g);
+  u = warp_sum(u);
+  if (lane != 0) return;
+  if constexpr (E4M3) {
+    const float xs = *p.x_scale;
+    g *= xs * p.g_scale[f];
+    u *= xs * p.u_scale[f];
+  }
+  h[f] = static_cast<uint16_t>(pack2<BF16>(act_value(g, p.act) * u, 0.f) & 0xffffu);
+}
+
 // ------------------------------------------------------------ tile orders ---
 
 // Row blocks in groups of GT_GROUP, column blocks across, row blocks of the group fastest: the
@@ -89,33 +171,17 @@ __device__ __forceinline__ void grouped_tile(int u, int num_m, int num_n, int& m
   m = m0 + (r - n * gm);
 }
 
-template <bool PAIR>
-struct GatedCfg {
-  static constexpr int TOK = PAIR ? 256 : 128;  // tokens per tile
-  static constexpr int FT = PAIR ? 128 : 64;    // features per tile
-};
+constexpr int GP_TOK = 256;  // pair tile: tokens
+constexpr int GP_FT = 128;   // pair tile: features
 
 // ---------------------------------------------------------------- forward ---
 
-template <bool E4M3, bool PAIR>
-__device__ __forceinline__ void gated_umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  if constexpr (PAIR && E4M3)
-    umma_f8_ss_pair(d, a, b, idesc, acc);
-  else if constexpr (PAIR)
-    umma_f16_ss_pair(d, a, b, idesc, acc);
-  else if constexpr (E4M3)
-    umma_f8_ss(d, a, b, idesc, acc);
-  else
-    umma_f16_ss(d, a, b, idesc, acc);
-}
-
 // BF16: the type of 16-bit operands and of h. The stage rows are 256 bytes whatever the type.
-template <bool BF16, bool E4M3, bool PAIR, bool SAVE>
+template <bool BF16, bool E4M3, bool SAVE>
 __global__ void __launch_bounds__(P_THREADS, 1)
     gated_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
                      const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_h,
                      const GatedParams p) {
-  using C = GatedCfg<PAIR>;
   constexpr int KB = E4M3 ? 2 * P_KB : P_KB;  // K per stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -129,10 +195,9 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_rank() : 0u;
-  const int unit0 = PAIR ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
-  const int step = PAIR ? static_cast<int>(cluster_count_x()) : static_cast<int>(gridDim.x);
-  const int num_m = (p.N + C::TOK - 1) / C::TOK, num_n = (p.F + C::FT - 1) / C::FT;
+  const uint32_t rank = cluster_rank();
+  const int unit0 = static_cast<int>(cluster_id_x()), step = static_cast<int>(cluster_count_x());
+  const int num_m = (p.N + GP_TOK - 1) / GP_TOK, num_n = (p.F + GP_FT - 1) / GP_FT;
   const int total = num_m * num_n;
   const int nkb = (p.H + KB - 1) / KB;
 
@@ -143,7 +208,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull_bar[b], 1);
-      mbar_init(&tempty_bar[b], (PAIR ? 2 : 1) * P_EPI);
+      mbar_init(&tempty_bar[b], 2 * P_EPI);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -156,17 +221,12 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     tma_prefetch_desc(&map_h);
   }
   if (warp == 1) {
-    if constexpr (PAIR) {
-      tmem_alloc_pair(tmem_holder, TMEM_COLS);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(tmem_holder, TMEM_COLS);
-      tmem_relinquish();
-    }
+    tmem_alloc_pair(tmem_holder, TMEM_COLS);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   const uint64_t tlimit = p.timeout_ns;
@@ -177,7 +237,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint32_t full_leader = PAIR ? mapa_shared(smem_u32(full_bar), 0) : 0u;
+      const uint32_t full_leader = mapa_shared(smem_u32(full_bar), 0);
       const CUtensorMap* map_b = rank == 0 ? &map_g : &map_u;
       for (int u = unit0; ok && u < total; u += step) {
         int m, n;
@@ -189,17 +249,10 @@ __global__ void __launch_bounds__(P_THREADS, 1)
           }
           uint8_t* sa = smem + stage * P_STAGE_BYTES;
           uint8_t* sb = sa + P_A_BYTES;
-          if constexpr (PAIR) {
-            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * P_STAGE_BYTES);
-            const uint32_t fb = full_leader + 8u * stage;
-            tma_load_3d_pair(sa, &map_x, fb, 0, m * C::TOK + BM * static_cast<int>(rank), 2 * kb);
-            tma_load_3d_pair(sb, map_b, fb, 0, n * C::FT, 2 * kb);
-          } else {
-            mbar_arrive_expect_tx(&full_bar[stage], P_STAGE_BYTES);
-            tma_load_3d(sa, &map_x, &full_bar[stage], 0, m * C::TOK, 2 * kb);
-            tma_load_3d(sb, &map_g, &full_bar[stage], 0, n * C::FT, 2 * kb);
-            tma_load_3d(sb + P_B_BYTES / 2, &map_u, &full_bar[stage], 0, n * C::FT, 2 * kb);
-          }
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * P_STAGE_BYTES);
+          const uint32_t fb = full_leader + 8u * stage;
+          tma_load_3d_pair(sa, &map_x, fb, 0, m * GP_TOK + BM * static_cast<int>(rank), 2 * kb);
+          tma_load_3d_pair(sb, map_b, fb, 0, n * GP_FT, 2 * kb);
           ++issued;
           if (++stage == P_STAGES) {
             stage = 0;
@@ -229,10 +282,9 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     // -------------------------------------------------------- UMMA issuer ---
     if (lane == 0 && rank == 0) {
       // kind::f8f6f4's e4m3 has the format code that kind::f16 gives to f16
-      constexpr uint32_t idesc =
-          make_idesc_f16(BF16 && !E4M3, false, false, PAIR ? 2 * BM : BM, PAIR ? 2 * C::FT : C::FT);
-      const uint32_t peer_empty = PAIR ? mapa_shared(smem_u32(empty_bar), 1) : 0u;
-      const uint32_t peer_tfull = PAIR ? mapa_shared(smem_u32(tfull_bar), 1) : 0u;
+      constexpr uint32_t idesc = make_idesc_f16(BF16 && !E4M3, false, false, 2 * BM, 2 * GP_FT);
+      const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
+      const uint32_t peer_tfull = mapa_shared(smem_u32(tfull_bar), 1);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -255,36 +307,23 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t accumulate = (kb | k) != 0 ? 1u : 0u;
-            if constexpr (PAIR) {
-              gated_umma<E4M3, true>(d_tmem, pair_operand_desc(sa, false, k), pair_operand_desc(sb, false, k), idesc,
-                                     accumulate);
-            } else {
-              // B: 64 rows per projection, their two 128-byte column blocks 8 KB apart
-              const uint32_t off = (k >> 2) * (BLOCK128_BYTES / 2) + (k & 3) * (UMMA_K * 2);
-              const uint64_t a = pair_operand_desc(sa, false, k);
-              gated_umma<E4M3, false>(d_tmem, a, smem_desc_sw128(sb + off, 16, 1024), idesc, accumulate);
-              gated_umma<E4M3, false>(d_tmem + 128, a, smem_desc_sw128(sb + P_B_BYTES / 2 + off, 16, 1024), idesc,
-                                      accumulate);
-            }
+            if constexpr (E4M3)
+              umma_f8_ss_pair(d_tmem, pair_operand_desc(sa, false, k), pair_operand_desc(sb, false, k), idesc,
+                              accumulate);
+            else
+              umma_f16_ss_pair(d_tmem, pair_operand_desc(sa, false, k), pair_operand_desc(sb, false, k), idesc,
+                               accumulate);
           }
-          if constexpr (PAIR) {
-            umma_commit_pair(smem_u32(&empty_bar[stage]));
-            umma_commit_pair(peer_empty + 8u * stage);
-          } else {
-            umma_commit(&empty_bar[stage]);
-          }
+          umma_commit_pair(smem_u32(&empty_bar[stage]));
+          umma_commit_pair(peer_empty + 8u * stage);
           if (++stage == P_STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        if constexpr (PAIR) {
-          umma_commit_pair(smem_u32(&tfull_bar[acc]));
-          umma_commit_pair(peer_tfull + 8u * acc);
-        } else {
-          umma_commit(&tfull_bar[acc]);
-        }
+        umma_commit_pair(smem_u32(&tfull_bar[acc]));
+        umma_commit_pair(peer_tfull + 8u * acc);
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1u;
@@ -294,10 +333,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
         raise_error(p.err, ERR_TIMEOUT);
         *abort_flag = 1;
       }
-      if constexpr (PAIR)
-        umma_commit_pair(smem_u32(drain_bar));
-      else
-        umma_commit(drain_bar);
+      umma_commit_pair(smem_u32(drain_bar));
       volatile int no_abort = 0;
       mbar_wait(drain_bar, 0, &no_abort, tlimit);
     }
@@ -307,7 +343,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     const int ch = (warp - 2) >> 2;  // half of the tile's features this warp handles
     uint8_t* xstage = smem + P_STAGES * P_STAGE_BYTES + 1024 + (warp - 2) * P_SLICE_BYTES;
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t leader_tempty = PAIR ? mapa_shared(smem_u32(tempty_bar), 0) : 0u;
+    const uint32_t leader_tempty = mapa_shared(smem_u32(tempty_bar), 0);
     const int fblocks = p.F / 32;
     int acc = 0, half = 0;
     uint32_t acc_phase = 0;
@@ -315,7 +351,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
     for (int u = unit0; u < total; u += step) {
       int m, n;
       grouped_tile(u, num_m, num_n, m, n);
-      const int row0 = m * C::TOK + BM * static_cast<int>(rank) + q * 32;  // this warp's first token
+      const int row0 = m * GP_TOK + BM * static_cast<int>(rank) + q * 32;  // this warp's first token
       float xs = 0.f;
       if constexpr (E4M3) xs = row0 + lane < p.N ? p.x_scale[row0 + lane] : 0.f;
       if (!mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, tlimit)) {
@@ -325,8 +361,8 @@ __global__ void __launch_bounds__(P_THREADS, 1)
       tc_fence_after();
       const uint32_t taddr = tmem_base + lane_base + static_cast<uint32_t>(acc * BN);
 #pragma unroll 1
-      for (int c = ch * (C::FT / 64); c < (ch + 1) * (C::FT / 64); ++c) {
-        const int f0 = n * C::FT + c * 32;
+      for (int c = ch * (GP_FT / 64); c < (ch + 1) * (GP_FT / 64); ++c) {
+        const int f0 = n * GP_FT + c * 32;
         uint32_t rg[32], ru[32];
         __syncwarp();
         tmem_ld_32x32b_x32(taddr + c * 32, rg);
@@ -379,10 +415,7 @@ __global__ void __launch_bounds__(P_THREADS, 1)
         }
       }
       tc_fence_before();
-      if constexpr (PAIR)
-        mbar_arrive_cluster(leader_tempty + 8u * acc);
-      else
-        mbar_arrive(&tempty_bar[acc]);
+      mbar_arrive_cluster(leader_tempty + 8u * acc);
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1u;
@@ -397,58 +430,304 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();
+  cluster_sync();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
-    if constexpr (PAIR)
-      tmem_dealloc_pair(tmem_base, TMEM_COLS);
-    else
-      tmem_dealloc(tmem_base, TMEM_COLS);
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------ forward, up to 128 tokens ---
+
+// One CTA per 64 features and all tokens: here the weights' read is all that counts, so they are
+// the A operand (64 gate rows and 64 up rows, M = 128) and the tokens the narrow B operand
+// (N = b_rows, the tokens rounded up to 16). With the tokens as A (M = 128 whatever their
+// number, one UMMA of N = 64 per projection) the UMMAs themselves read 6 KB of shared memory per
+// 4 KB of weights and held every SM to 21 bytes of weights per clock (one B200: 3584 x 18944 in
+// 16 bits 47 us, 4096 x 14336, whose 224 tiles leave 72 SMs idle in the second round, 53 us).
+// Boxes end with the tokens there are: one whose rows lie mostly outside its tensor arrives
+// later than one that is read (72 us for 1 token in 128-row boxes against 50 us for 64).
+// A stage is K = 128 (256 for e4m3): per 128-byte column block the gate rows and the up rows
+// follow one another, four 8 KB boxes. Lanes 0-63 of the accumulator are gate features, 64-127
+// the same features of up: the up warps hand their values over through shared memory.
+constexpr int GF_FT = 64;
+constexpr int GF_W_BYTES = 2 * GF_FT * 2 * 128;          // 32 KB of weights per stage
+constexpr int GF_MAX_STAGES = 5;
+constexpr int GF_STAGE_AREA = P_STAGES * P_STAGE_BYTES;  // shared memory for stages
+constexpr int GF_XCH_PITCH = 17;                         // floats per feature of a handed-over block
+
+template <bool BF16, bool E4M3, bool SAVE>
+__global__ void __launch_bounds__(P_THREADS, 1)
+    gated_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g,
+                     const __grid_constant__ CUtensorMap map_u, uint16_t* __restrict__ h, const GatedParams p) {
+  constexpr int KB = E4M3 ? 2 * P_KB : P_KB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = GF_W_BYTES + p.b_rows * 256;
+  const int stages = min(GF_MAX_STAGES, GF_STAGE_AREA / stage_bytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + GF_STAGE_AREA);
+  uint64_t* empty_bar = full_bar + GF_MAX_STAGES;
+  uint64_t* tfull_bar = empty_bar + GF_MAX_STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const int total = p.F / GF_FT;
+  const int nkb = (p.H + KB - 1) / KB;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], P_EPI);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_g);
+    tma_prefetch_desc(&map_u);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const uint64_t tlimit = p.timeout_ns;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int n = blockIdx.x; ok && n < total; n += gridDim.x) {
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, tlimit)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sw = smem + stage * stage_bytes;
+          mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            tma_load_3d(sw + z * (GF_W_BYTES / 2), &map_g, &full_bar[stage], 0, n * GF_FT, 2 * kb + z);
+            tma_load_3d(sw + z * (GF_W_BYTES / 2) + GF_W_BYTES / 4, &map_u, &full_bar[stage], 0, n * GF_FT,
+                        2 * kb + z);
+          }
+          tma_load_3d(sw + GF_W_BYTES, &map_x, &full_bar[stage], 0, 0, 2 * kb);
+          ++issued;
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+        const int outstanding = issued < stages ? issued : stages;
+        for (int i = 1; i <= outstanding; ++i) {
+          int s = stage - i;
+          uint32_t ph = phase;
+          if (s < 0) {
+            s += stages;
+            ph ^= 1u;
+          }
+          volatile int no_abort = 0;
+          mbar_wait(&full_bar[s], ph, &no_abort, tlimit);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // N of the instruction is the launch's: uniform for all threads, computed once
+      const uint32_t idesc = make_idesc_f16(BF16 && !E4M3, false, false, BM, p.b_rows);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int n = blockIdx.x; ok && n < total; n += gridDim.x) {
+        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, tlimit)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 128);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag, tlimit)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sw = smem_u32(smem + stage * stage_bytes), sx = sw + GF_W_BYTES;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t step = (k & 3) * (UMMA_K * 2);
+            const uint64_t a = smem_desc_sw128(sw + (k >> 2) * (GF_W_BYTES / 2) + step, 16, 1024);
+            const uint64_t b = smem_desc_sw128(sx + (k >> 2) * (p.b_rows * 128) + step, 16, 1024);
+            if constexpr (E4M3)
+              umma_f8_ss(d_tmem, a, b, idesc, (kb | k) != 0 ? 1u : 0u);
+            else
+              umma_f16_ss(d_tmem, a, b, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          umma_commit(&empty_bar[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tfull_bar[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok) {
+        raise_error(p.err, ERR_TIMEOUT);
+        *abort_flag = 1;
+      }
+      umma_commit(drain_bar);
+      volatile int no_abort = 0;
+      mbar_wait(drain_bar, 0, &no_abort, tlimit);
+    }
+  } else {
+    // Two groups of four warps take the 32-token column chunks in turn; in each, warps of lane
+    // quadrants 0 and 1 hold gate, 2 and 3 up.
+    const int q = warp & 3, grp = (warp - 2) >> 2;
+    const bool is_gate = q < 2;
+    float* blocks = reinterpret_cast<float*>(smem + GF_STAGE_AREA + 1024) + grp * (2 * GF_FT * GF_XCH_PITCH) +
+                    ((q & 1) * 32 + lane) * GF_XCH_PITCH;
+    float* give = blocks + (is_gate ? 0 : GF_FT * GF_XCH_PITCH);
+    const float* take = blocks + (is_gate ? GF_FT * GF_XCH_PITCH : 0);
+    const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int n = blockIdx.x; n < total; n += gridDim.x) {
+      const int f = n * GF_FT + (q & 1) * 32 + lane;
+      float scale = 1.f;
+      if constexpr (E4M3) scale = is_gate ? p.g_scale[f] : p.u_scale[f];
+      if (!mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, tlimit)) ok = false;
+      // the four warps of a group leave the loop together: the barriers below count all of them
+      if (!(grp == 0 ? named_bar_all<1, 128>(ok) : named_bar_all<2, 128>(ok))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + lane_base + static_cast<uint32_t>(acc * 128);
+      for (int t0 = grp * 32; t0 < p.N; t0 += 64) {
+        uint32_t raw[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + t0, raw);
+        tmem_ld_wait(raw);
+        float own[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          own[j] = __uint_as_float(is_gate ? raw[j] : raw[16 + j]) * scale;
+          give[j] = __uint_as_float(is_gate ? raw[16 + j] : raw[j]) * scale;
+        }
+        grp == 0 ? named_bar<1, 128>() : named_bar<2, 128>();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int t = t0 + j + (is_gate ? 0 : 16);
+          if (t < p.N) {
+            const float other = take[j];
+            float g = is_gate ? own[j] : other, u = is_gate ? other : own[j];
+            if constexpr (E4M3) {
+              const float xs = __ldg(p.x_scale + t);
+              g *= xs;
+              u *= xs;
+            }
+            if constexpr (SAVE) {
+              float* sv = p.saved + (static_cast<size_t>(t / 32) * (p.F / 32) + f / 32) * (2 * GATED_SAVE_BLOCK) +
+                          (f % 32) / 4 * 128 + (t % 32) * 4 + f % 4;
+              sv[0] = g;
+              sv[GATED_SAVE_BLOCK] = u;
+            }
+            h[static_cast<size_t>(t) * p.F + f] =
+                static_cast<uint16_t>(pack2<BF16>(act_value(g, p.act) * u, 0.f) & 0xffffu);
+          }
+        }
+        grp == 0 ? named_bar<1, 128>() : named_bar<2, 128>();
+      }
+      tc_fence_before();
+      mbar_arrive(&tempty_bar[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    if (!ok) {
+      raise_error(p.err, ERR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, BN);
   }
 }
 
 // --------------------------------------------------- backward: dg and du ---
 
-// One warp per 32 tokens x 32 features of the saved blocks: g and u arrive as they were stored
-// (512 contiguous bytes per load), dh and the results pass through an 80-byte-pitch row staging
-// (conflict-free for 16-byte accesses by row and by column group). Memory-bound: 14 bytes per
-// element.
+// One warp per 32 tokens x 32 features of the saved blocks, 16 features at a time: g and u
+// arrive as they were stored (512 contiguous bytes per load), dh and the results pass through a
+// 48-byte-pitch row staging (conflict-free for 16-byte accesses by row and by column pair).
+// Memory-bound, 14 bytes per element: halves of 16 features keep a thread under 64 registers, so
+// that 32 warps per SM cover each other's loads.
 constexpr int GATED_DACT_WARPS = 4;
 template <bool BF16>
-__global__ void __launch_bounds__(32 * GATED_DACT_WARPS)
+__global__ void __launch_bounds__(32 * GATED_DACT_WARPS, 8)
     gated_dact_kernel(const float4* __restrict__ saved, const uint4* __restrict__ dh, int n, int f, int act,
                       uint4* __restrict__ dg, uint4* __restrict__ du) {
-  __shared__ uint4 st[GATED_DACT_WARPS][32][5];
+  __shared__ uint4 st[GATED_DACT_WARPS][32][3];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int fb = f / 32, vec = f / 8;
-  const long long blocks = static_cast<long long>((n + 31) / 32) * fb;
-  for (long long b = static_cast<long long>(blockIdx.x) * GATED_DACT_WARPS + warp; b < blocks;
+  const long long halves = static_cast<long long>((n + 31) / 32) * fb * 2;
+  const int r0 = lane >> 1, c = lane & 1;
+  for (long long b = static_cast<long long>(blockIdx.x) * GATED_DACT_WARPS + warp; b < halves;
        b += static_cast<long long>(gridDim.x) * GATED_DACT_WARPS) {
-    const int rb = static_cast<int>(b / fb), cb = static_cast<int>(b - static_cast<long long>(rb) * fb);
-    const float4* sv = saved + b * (2 * GATED_SAVE_BLOCK / 4) + lane;
-    float4 g[8], u[8];
+    const long long blk = b >> 1;
+    const int h = static_cast<int>(b & 1);
+    const int rb = static_cast<int>(blk / fb), cb = static_cast<int>(blk - static_cast<long long>(rb) * fb);
+    const float4* sv = saved + blk * (2 * GATED_SAVE_BLOCK / 4) + h * 128 + lane;
+    const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 4 + h * 2 + c;
+    const bool live0 = rb * 32 + r0 < n, live1 = rb * 32 + r0 + 16 < n;
+    float4 g[4], u[4];
+    uint4 d0 = make_uint4(0u, 0u, 0u, 0u), d1 = d0;
+    if (live0) d0 = __ldcs(dh + at);
+    if (live1) d1 = __ldcs(dh + at + 16ll * vec);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = __ldcs(sv + j * 32);
+    for (int j = 0; j < 4; ++j) g[j] = __ldcs(sv + j * 32);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = __ldcs(sv + 256 + j * 32);
-    const int c = lane & 3;
-    __syncwarp();  // the last block's rows have left the staging
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      const long long row = static_cast<long long>(rb) * 32 + r;
-      st[warp][r][c] = row < n ? __ldcs(dh + row * vec + cb * 4 + c) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int j = 0; j < 4; ++j) u[j] = __ldcs(sv + 256 + j * 32);
+    __syncwarp();  // the last rows have left the staging
+    st[warp][r0][c] = d0;
+    st[warp][r0 + 16][c] = d1;
     __syncwarp();
-    float d[32];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) unpack8<BF16>(st[warp][lane][i], d + 8 * i);
+    float d[16], e[16];
+    unpack8<BF16>(st[warp][lane][0], d);
+    unpack8<BF16>(st[warp][lane][1], d + 8);
     const float* gf = reinterpret_cast<const float*>(g);
     const float* uf = reinterpret_cast<const float*>(u);
-    float e[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < 16; ++j) {
       float a, da;
       act_both(gf[j], act, a, da);
       e[j] = d[j] * a;
@@ -457,15 +736,12 @@ __global__ void __launch_bounds__(32 * GATED_DACT_WARPS)
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st[warp][lane][i] = pack8<BF16>((pass ? e : d) + 8 * i);
+      st[warp][lane][0] = pack8<BF16>(pass ? e : d);
+      st[warp][lane][1] = pack8<BF16>((pass ? e : d) + 8);
       __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        const long long row = static_cast<long long>(rb) * 32 + r;
-        if (row < n) (pass ? du : dg)[row * vec + cb * 4 + c] = st[warp][r][c];
-      }
+      uint4* out = pass ? du : dg;
+      if (live0) out[at] = st[warp][r0][c];
+      if (live1) out[at + 16ll * vec] = st[warp][r0 + 16][c];
     }
   }
 }

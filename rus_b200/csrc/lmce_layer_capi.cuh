@@ -160,28 +160,49 @@ int make_map_3d_bytes(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
   return LMCE_OK;
 }
 
-template <bool BF16, bool E4M3, bool PAIR, bool SAVE>
-int launch_gated(const CUtensorMap* maps, const GatedParams& p, int sms, cudaStream_t st) {
-  using C = GatedCfg<PAIR>;
-  auto kern = gated_fwd_kernel<BF16, E4M3, PAIR, SAVE>;
+// maps: x, gate, up, h
+template <bool BF16, bool E4M3, bool SAVE>
+int launch_gated_pairs(const CUtensorMap* maps, const GatedParams& p, int sms, cudaStream_t st) {
+  auto kern = gated_fwd_kernel<BF16, E4M3, SAVE>;
   static bool done[kMaxDevices] = {};
   if (int rc = ensure_smem_attr(kern, PBWD_SMEM_BYTES, done)) return rc;
   static int cache[kMaxDevices] = {};
-  const int slots = PAIR ? max_pairs(kern, PBWD_SMEM_BYTES, sms, cache, P_THREADS) : sms;
-  const int64_t units = static_cast<int64_t>((p.N + C::TOK - 1) / C::TOK) * ((p.F + C::FT - 1) / C::FT);
-  const int grid = static_cast<int>(std::min<int64_t>(units, slots)) * (PAIR ? 2 : 1);
-  return launch_ex(kern, grid, P_THREADS, PBWD_SMEM_BYTES, PAIR ? 2 : 1, st, maps[0], maps[1], maps[2], maps[3], p);
+  const int slots = max_pairs(kern, PBWD_SMEM_BYTES, sms, cache, P_THREADS);
+  const int64_t units = static_cast<int64_t>((p.N + GP_TOK - 1) / GP_TOK) * ((p.F + GP_FT - 1) / GP_FT);
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(units, slots));
+  return launch_ex(kern, grid, P_THREADS, PBWD_SMEM_BYTES, 2, st, maps[0], maps[1], maps[2], maps[3], p);
+}
+
+template <bool BF16, bool E4M3, bool SAVE>
+int launch_gated_few(const CUtensorMap* maps, const GatedParams& p, void* h, int sms, cudaStream_t st) {
+  auto kern = gated_few_kernel<BF16, E4M3, SAVE>;
+  static bool done[kMaxDevices] = {};
+  if (int rc = ensure_smem_attr(kern, PBWD_SMEM_BYTES, done)) return rc;
+  const int grid = std::min(p.F / GF_FT, sms);
+  return launch_ex(kern, grid, P_THREADS, PBWD_SMEM_BYTES, 1, st, maps[0], maps[1], maps[2], static_cast<uint16_t*>(h),
+                   p);
 }
 
 template <bool BF16, bool E4M3>
-int launch_gated_any(const CUtensorMap* maps, const GatedParams& p, bool pair, int sms, cudaStream_t st) {
+int launch_gated(const CUtensorMap* maps, const GatedParams& p, void* h, int sms, cudaStream_t st) {
+  const bool pairs = p.N > BM;
   if constexpr (!E4M3) {
     if (p.saved != nullptr)
-      return pair ? launch_gated<BF16, E4M3, true, true>(maps, p, sms, st)
-                  : launch_gated<BF16, E4M3, false, true>(maps, p, sms, st);
+      return pairs ? launch_gated_pairs<BF16, E4M3, true>(maps, p, sms, st)
+                   : launch_gated_few<BF16, E4M3, true>(maps, p, h, sms, st);
   }
-  return pair ? launch_gated<BF16, E4M3, true, false>(maps, p, sms, st)
-              : launch_gated<BF16, E4M3, false, false>(maps, p, sms, st);
+  return pairs ? launch_gated_pairs<BF16, E4M3, false>(maps, p, sms, st)
+               : launch_gated_few<BF16, E4M3, false>(maps, p, h, sms, st);
+}
+
+template <bool BF16, bool E4M3>
+int launch_gated_token(const void* x, const void* wg, const void* wu, const GatedParams& p, void* h,
+                       cudaStream_t st) {
+  const int vec = p.H / (E4M3 ? 16 : 8), grid = (p.F + GT_WARPS - 1) / GT_WARPS;
+  gated_token_kernel<BF16, E4M3><<<grid, 32 * GT_WARPS, 0, st>>>(
+      static_cast<const uint4*>(x), static_cast<const uint4*>(wg), static_cast<const uint4*>(wu), vec, p,
+      static_cast<uint16_t*>(h));
+  return launched();
 }
 
 int check_gated(int64_t n, int64_t h, int64_t f, int dtype, int act, int64_t h_step) {
@@ -382,12 +403,7 @@ int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64
   if (int rc = device_info(&d)) return rc;
   if (int rc = get_encoder()) return rc;
   const bool bf16 = dtype == LMCE_DTYPE_BF16, pair = n_rows > BM;
-  const uint32_t w_rows = pair ? 128 : 64;
-  CUtensorMap maps[4];
-  if (int rc = make_map_3d(&maps[0], x, bf16, hidden_dim, n_rows, hidden_dim, 128, 2)) return rc;
-  if (int rc = make_map_3d(&maps[1], w_gate, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, 2)) return rc;
-  if (int rc = make_map_3d(&maps[2], w_up, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, 2)) return rc;
-  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   GatedParams p = {};
   p.N = static_cast<int>(n_rows);
   p.H = static_cast<int>(hidden_dim);
@@ -396,9 +412,19 @@ int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64
   p.saved = static_cast<float*>(saved);
   p.err = d->err_ptr;
   p.timeout_ns = wait_timeout_ns();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return bf16 ? launch_gated_any<true, false>(maps, p, pair, d->sms, st)
-              : launch_gated_any<false, false>(maps, p, pair, d->sms, st);
+  if (n_rows == 1 && !saved)
+    return bf16 ? launch_gated_token<true, false>(x, w_gate, w_up, p, h_out, st)
+                : launch_gated_token<false, false>(x, w_gate, w_up, p, h_out, st);
+  const uint32_t x_rows = pair ? 128 : static_cast<uint32_t>((n_rows + 15) / 16 * 16);
+  const uint32_t w_rows = pair ? 128 : 64, w_blocks = pair ? 2 : 1;
+  p.b_rows = static_cast<int>(x_rows);
+  CUtensorMap maps[4];
+  if (int rc = make_map_3d(&maps[0], x, bf16, hidden_dim, n_rows, hidden_dim, x_rows, 2)) return rc;
+  if (int rc = make_map_3d(&maps[1], w_gate, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, w_blocks)) return rc;
+  if (int rc = make_map_3d(&maps[2], w_up, bf16, hidden_dim, ffn_dim, hidden_dim, w_rows, w_blocks)) return rc;
+  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
+  return bf16 ? launch_gated<true, false>(maps, p, h_out, d->sms, st)
+              : launch_gated<false, false>(maps, p, h_out, d->sms, st);
 }
 
 int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const void* w_gate, const float* gate_scale,
@@ -414,12 +440,6 @@ int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const void* w_ga
   if (int rc = device_info(&d)) return rc;
   if (int rc = get_encoder()) return rc;
   const bool bf16 = out_dtype == LMCE_DTYPE_BF16, pair = n_rows > BM;
-  const uint32_t w_rows = pair ? 128 : 64;
-  CUtensorMap maps[4];
-  if (int rc = make_map_3d_bytes(&maps[0], x, hidden_dim, n_rows, 128, 2)) return rc;
-  if (int rc = make_map_3d_bytes(&maps[1], w_gate, hidden_dim, ffn_dim, w_rows, 2)) return rc;
-  if (int rc = make_map_3d_bytes(&maps[2], w_up, hidden_dim, ffn_dim, w_rows, 2)) return rc;
-  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
   GatedParams p = {};
   p.N = static_cast<int>(n_rows);
   p.H = static_cast<int>(hidden_dim);
@@ -431,8 +451,19 @@ int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const void* w_ga
   p.err = d->err_ptr;
   p.timeout_ns = wait_timeout_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return bf16 ? launch_gated_any<true, true>(maps, p, pair, d->sms, st)
-              : launch_gated_any<false, true>(maps, p, pair, d->sms, st);
+  if (n_rows == 1)
+    return bf16 ? launch_gated_token<true, true>(x, w_gate, w_up, p, h_out, st)
+                : launch_gated_token<false, true>(x, w_gate, w_up, p, h_out, st);
+  const uint32_t x_rows = pair ? 128 : static_cast<uint32_t>((n_rows + 15) / 16 * 16);
+  const uint32_t w_rows = pair ? 128 : 64, w_blocks = pair ? 2 : 1;
+  p.b_rows = static_cast<int>(x_rows);
+  CUtensorMap maps[4];
+  if (int rc = make_map_3d_bytes(&maps[0], x, hidden_dim, n_rows, x_rows, 2)) return rc;
+  if (int rc = make_map_3d_bytes(&maps[1], w_gate, hidden_dim, ffn_dim, w_rows, w_blocks)) return rc;
+  if (int rc = make_map_3d_bytes(&maps[2], w_up, hidden_dim, ffn_dim, w_rows, w_blocks)) return rc;
+  if (int rc = make_map_store16(&maps[3], h_out, bf16, ffn_dim, n_rows, ffn_dim)) return rc;
+  return bf16 ? launch_gated<true, true>(maps, p, h_out, d->sms, st)
+              : launch_gated<false, true>(maps, p, h_out, d->sms, st);
 }
 
 size_t lmce_gated_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int want_dx,
@@ -463,9 +494,9 @@ int lmce_gated_backward(const void* d_h, const void* saved, const void* x, const
   const int64_t n = n_rows, h = hidden_dim, f = ffn_dim;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
-  const int64_t blocks = (n + 31) / 32 * (f / 32);
+  const int64_t halves = (n + 31) / 32 * (f / 16);
   const int dgrid = static_cast<int>(
-      std::min<int64_t>((blocks + GATED_DACT_WARPS - 1) / GATED_DACT_WARPS, d->sms * 16ll));
+      std::min<int64_t>((halves + GATED_DACT_WARPS - 1) / GATED_DACT_WARPS, d->sms * 8ll));
   if (bf16)
     gated_dact_kernel<true><<<dgrid, 32 * GATED_DACT_WARPS, 0, st>>>(
         static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),

@@ -9,32 +9,35 @@ follows is one plain product. CUDA tensors only: there is no CPU path.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .norm import _rows
-from .ops import _DTYPES, _ptr, _stream
+from .norm import _rows, no_second_order
+from .ops import _DTYPES, _ptr
 
 ACTIVATIONS = {"silu": _lib.LMCE_ACT_SILU, "gelu_tanh": _lib.LMCE_ACT_GELU_TANH}
 
 
 def _check(x, w_gate, w_up, activation, who: str, step: int) -> None:
+    dt, dev, shape = x.dtype, x.device, w_gate.shape
+    if (activation in ACTIVATIONS and dev.type == "cuda" and w_gate.device == dev and w_up.device == dev
+            and w_gate.dtype == dt and w_up.dtype == dt and len(shape) == 2 and w_up.shape == shape and x.dim() > 0
+            and x.shape[-1] == shape[1] and shape[0] > 0 and shape[0] % 64 == 0 and shape[1] > 0
+            and shape[1] % step == 0):
+        return
     if activation not in ACTIVATIONS:
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
                              f"{who}: activation {activation!r} (need one of {sorted(ACTIVATIONS)})")
     if not (x.is_cuda and w_gate.is_cuda and w_up.is_cuda):
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who} runs on CUDA tensors only (no CPU path)")
-    if x.dim() == 0 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
+    if x.dim() == 0 or w_gate.dim() != 2 or w_up.shape != shape or shape[1] != x.shape[-1]:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT,
                              f"{who}: both weights must be [F, H] with H = x.shape[-1]")
-    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+    if w_gate.dtype != dt or w_up.dtype != dt:
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who}: x and both weights must have the same dtype")
-    if w_gate.device != x.device or w_up.device != x.device:
+    if w_gate.device != dev or w_up.device != dev:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: all tensors must be on the same device")
-    f, h = w_gate.shape
-    if f <= 0 or f % 64 or h <= 0 or h % step:
-        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
-                             f"{who}: sizes H={h}, F={f} (need H a multiple of {step}, F of 64)")
+    raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
+                         f"{who}: sizes H={shape[1]}, F={shape[0]} (need H a multiple of {step}, F of 64)")
 
 
 def _forward(x, w_gate, w_up, activation, save: bool):
@@ -44,12 +47,10 @@ def _forward(x, w_gate, w_up, activation, save: bool):
     out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=x.device)
     saved = None
     if n > 0:
-        with torch.cuda.device(x.device):
-            if save:
-                saved = torch.empty(int(_lib.load().lmce_gated_saved_bytes(n, f)), dtype=torch.uint8,
-                                    device=x.device)
-            _lib.call("lmce_gated_linear", xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), n, h, f, _DTYPES[x.dtype],
-                      ACTIVATIONS[activation], out.data_ptr(), _ptr(saved), _stream(x.device))
+        if save:
+            saved = torch.empty(int(_lib.load().lmce_gated_saved_bytes(n, f)), dtype=torch.uint8, device=x.device)
+        _lib.launch(x.device, "lmce_gated_linear", xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), n, h, f,
+                    _DTYPES[x.dtype], ACTIVATIONS[activation], out.data_ptr(), _ptr(saved))
     return out, xc, wg, wu, saved
 
 
@@ -62,8 +63,8 @@ class GatedLinearFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh):
+        no_second_order("gated_linear")
         x, wg, wu, saved = ctx.saved_tensors
         want_x, want_g, want_u = ctx.needs_input_grad[:3]
         f, h = wg.shape
@@ -77,10 +78,9 @@ class GatedLinearFn(torch.autograd.Function):
             g = _rows(dh)
             ws_bytes = int(_lib.load().lmce_gated_bwd_workspace_bytes(n, h, f, want_x, want_g + want_u))
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            with torch.cuda.device(dev):
-                _lib.call("lmce_gated_backward", g.data_ptr(), saved.data_ptr(), x.data_ptr(), wg.data_ptr(),
-                          wu.data_ptr(), n, h, f, _DTYPES[x.dtype], ACTIVATIONS[ctx.activation], _ptr(dx), _ptr(dg),
-                          _ptr(du), ws.data_ptr(), ws_bytes, _stream(dev))
+            _lib.launch(dev, "lmce_gated_backward", g.data_ptr(), saved.data_ptr(), x.data_ptr(), wg.data_ptr(),
+                        wu.data_ptr(), n, h, f, _DTYPES[x.dtype], ACTIVATIONS[ctx.activation], _ptr(dx), _ptr(dg),
+                        _ptr(du), ws.data_ptr(), ws_bytes)
         return dx, dg, du, None
 
 
@@ -135,8 +135,7 @@ def gated_linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w_gate: torch.Tens
     n = xc.numel() // h
     out = torch.empty((*x.shape[:-1], f), dtype=out_dtype, device=x.device)
     if n > 0:
-        with torch.cuda.device(x.device):
-            _lib.call("lmce_gated_linear_e4m3", xc.data_ptr(), sx.data_ptr(), wg.data_ptr(), sg.data_ptr(),
-                      wu.data_ptr(), su.data_ptr(), n, h, f, _DTYPES[out_dtype], ACTIVATIONS[activation],
-                      out.data_ptr(), _stream(x.device))
+        _lib.launch(x.device, "lmce_gated_linear_e4m3", xc.data_ptr(), sx.data_ptr(), wg.data_ptr(), sg.data_ptr(),
+                    wu.data_ptr(), su.data_ptr(), n, h, f, _DTYPES[out_dtype], ACTIVATIONS[activation],
+                    out.data_ptr())
     return out

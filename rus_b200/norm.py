@@ -9,34 +9,44 @@ block. CUDA tensors only: there is no CPU path.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPES, _ptr, _stream
+from .ops import _DTYPES, _ptr
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous and on a 16-byte boundary (a copy where it is not)."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        return t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def no_second_order(who: str) -> None:
+    """In a backward: autograd runs it in grad mode only to differentiate it again."""
+    if torch.is_grad_enabled():
+        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who}: no second derivative (create_graph=True)")
+
+
 def _check(x, residual, weight, who: str) -> None:
+    dt, dev, shape = x.dtype, x.device, x.shape
+    if (dt in _DTYPES and dev.type == "cuda" and weight.dtype == dt and weight.device == dev and weight.dim() == 1
+            and shape and shape[-1] == weight.shape[0] and shape[-1] % 8 == 0 and 0 < shape[-1] <= 16384
+            and (residual is None or (residual.dtype == dt and residual.device == dev and residual.shape == shape))):
+        return
     if not x.is_cuda or not weight.is_cuda or (residual is not None and not residual.is_cuda):
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who} runs on CUDA tensors only (no CPU path)")
-    if x.dtype not in _DTYPES:
-        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who}: dtype {x.dtype} (need fp16 or bf16)")
-    if x.dim() == 0 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+    if dt not in _DTYPES:
+        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who}: dtype {dt} (need fp16 or bf16)")
+    if not shape or weight.dim() != 1 or weight.shape[0] != shape[-1]:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: weight must be [H] with H = x.shape[-1]")
-    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+    if weight.dtype != dt or (residual is not None and residual.dtype != dt):
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"{who}: x, residual and weight must have the same dtype")
-    if residual is not None and residual.shape != x.shape:
+    if residual is not None and residual.shape != shape:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: residual must have the shape of x")
-    if weight.device != x.device or (residual is not None and residual.device != x.device):
+    if weight.device != dev or (residual is not None and residual.device != dev):
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"{who}: all tensors must be on the same device")
-    if x.shape[-1] % 8 != 0 or not 0 < x.shape[-1] <= 16384:
-        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
-                             f"{who}: hidden size {x.shape[-1]} (need a multiple of 8, at most 16384)")
+    raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
+                         f"{who}: hidden size {shape[-1]} (need a multiple of 8, at most 16384)")
 
 
 def _forward(x, residual, weight, eps, keep_rstd: bool):
@@ -48,9 +58,8 @@ def _forward(x, residual, weight, eps, keep_rstd: bool):
     s = xc if rc is None else torch.empty_like(xc)
     rstd = torch.empty(n, dtype=torch.float32, device=x.device) if keep_rstd else None
     if n > 0:
-        with torch.cuda.device(x.device):
-            _lib.call("lmce_add_rmsnorm", xc.data_ptr(), _ptr(rc), w.data_ptr(), float(eps), n, h, _DTYPES[x.dtype],
-                      s.data_ptr(), y.data_ptr(), _ptr(rstd), _stream(x.device))
+        _lib.launch(x.device, "lmce_add_rmsnorm", xc.data_ptr(), _ptr(rc), w.data_ptr(), eps, n, h, _DTYPES[x.dtype],
+                    s.data_ptr(), y.data_ptr(), _ptr(rstd))
     return y, s, w, rstd
 
 
@@ -65,8 +74,8 @@ class AddRMSNormFn(torch.autograd.Function):
         return y if residual is None else (y, s)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, ds=None):
+        no_second_order("add_rms_norm")
         s, w, rstd = ctx.saved_tensors
         want_x, want_r, want_w = ctx.needs_input_grad[:3]
         if dy is None and ds is None:
@@ -83,10 +92,9 @@ class AddRMSNormFn(torch.autograd.Function):
             if want_dw:
                 ws_bytes = int(_lib.load().lmce_add_rmsnorm_bwd_workspace_bytes(n, h))
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            with torch.cuda.device(dev):
-                _lib.call("lmce_add_rmsnorm_backward", _ptr(g), _ptr(gs), s.data_ptr(), w.data_ptr(),
-                          rstd.data_ptr(), n, h, _DTYPES[s.dtype], _ptr(dx), dw.data_ptr() if want_dw else None,
-                          _ptr(ws), ws_bytes, _stream(dev))
+            _lib.launch(dev, "lmce_add_rmsnorm_backward", _ptr(g), _ptr(gs), s.data_ptr(), w.data_ptr(),
+                        rstd.data_ptr(), n, h, _DTYPES[s.dtype], _ptr(dx), dw.data_ptr() if want_dw else None,
+                        _ptr(ws), ws_bytes)
         return dx if want_x else None, dx if want_r else None, dw, None
 
 
@@ -128,7 +136,6 @@ def add_rms_norm_e4m3(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     s = xc if rc is None else torch.empty_like(xc)
     if n > 0:
-        with torch.cuda.device(x.device):
-            _lib.call("lmce_add_rmsnorm_e4m3", xc.data_ptr(), _ptr(rc), w.data_ptr(), float(eps), n, h,
-                      _DTYPES[x.dtype], s.data_ptr(), q.data_ptr(), scale.data_ptr(), _stream(x.device))
+        _lib.launch(x.device, "lmce_add_rmsnorm_e4m3", xc.data_ptr(), _ptr(rc), w.data_ptr(), eps, n, h,
+                    _DTYPES[x.dtype], s.data_ptr(), q.data_ptr(), scale.data_ptr())
     return q, scale, (x if residual is None else s)
