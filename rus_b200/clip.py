@@ -8,6 +8,7 @@ launches for up to 1024 gradients of any mix of fp16, bf16 and fp32.
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -15,6 +16,7 @@ from . import _lib
 
 _GRAD_DTYPES = {torch.float16: _lib.LMCE_DTYPE_F16, torch.bfloat16: _lib.LMCE_DTYPE_BF16,
                 torch.float32: _lib.LMCE_DTYPE_F32}
+_dtype_of = attrgetter("dtype")
 
 
 @torch.no_grad()
@@ -27,42 +29,44 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     one CUDA device, of any alignment (a non-contiguous one goes through a copy). They are
     multiplied by ``max_norm / (norm + 1e-6)`` where that is below 1 and left as they are
     otherwise; a norm that is not a number makes them all so, an infinite one zeroes the
-    finite ones, as in torch; ``max_norm=inf`` only measures. Nothing is read back to the host unless ``error_if_nonfinite``
-    asks for an error in those two cases (before any gradient changes)."""
+    finite ones, as in torch; ``max_norm=inf`` only measures. Nothing is read back to the host
+    unless ``error_if_nonfinite`` asks for an error in those two cases (before any gradient
+    changes)."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, f"clip_grad_norm_: max_norm {max_norm}")
-    grads = [g for g in [p.grad for p in params] if g is not None]
+    grads = [g for p in params if (g := p.grad) is not None]
     if not grads:
         return torch.zeros((), device=params[0].device if params else None)
-    # one attribute of all gradients at a time: with hundreds of small gradients the host's work
-    # on them is what the call costs
+    # one attribute of all gradients at a time, through C-level maps: with hundreds of small
+    # gradients the host's work on them is what the call costs
     dev = grads[0].device
     if dev.type != "cuda":
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, "clip_grad_norm_ runs on CUDA gradients only (no CPU path)")
-    if {g.layout for g in grads} != {torch.strided}:
-        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, "clip_grad_norm_: a sparse gradient (need dense ones)")
-    if {g.device for g in grads} != {dev}:
+    if set(map(torch.Tensor.get_device, grads)) != {dev.index}:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients on several devices")
-    kinds = [g.dtype for g in grads]
+    kinds = list(map(_dtype_of, grads))
     if not _GRAD_DTYPES.keys() >= set(kinds):
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
                              f"clip_grad_norm_: gradients of {set(kinds) - _GRAD_DTYPES.keys()} (need fp16, bf16, fp32)")
-    ptrs = [g.data_ptr() for g in grads]
+    try:
+        ptrs = list(map(torch.Tensor.data_ptr, grads))
+    except RuntimeError as e:  # no storage
+        raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"clip_grad_norm_: a gradient that is not dense ({e})") from e
     if len(set(ptrs)) < len(ptrs):  # a parameter listed twice counts once (empty gradients share address 0)
-        grads = [p.grad for p in dict.fromkeys(params) if p.grad is not None]
-        kinds, ptrs = [g.dtype for g in grads], [g.data_ptr() for g in grads]
+        grads = [g for p in dict.fromkeys(params) if (g := p.grad) is not None]
+        kinds, ptrs = list(map(_dtype_of, grads)), list(map(torch.Tensor.data_ptr, grads))
     copies = []
-    if not all([g.is_contiguous() for g in grads]):
+    if not all(map(torch.Tensor.is_contiguous, grads)):
         for i, g in enumerate(grads):
             if not g.is_contiguous():
                 c = g.contiguous()
                 copies.append((g, c))
                 ptrs[i] = c.data_ptr()
     count = len(grads)
-    table = array("q", ptrs + [g.numel() for g in grads])
-    codes = array("i", [_GRAD_DTYPES[k] for k in kinds])
+    table = array("q", ptrs + list(map(torch.Tensor.numel, grads)))
+    codes = array("i", map(_GRAD_DTYPES.__getitem__, kinds))
     at = table.buffer_info()[0]
     total = torch.empty((), dtype=torch.float32, device=dev)
     ws_bytes = int(_lib.load().lmce_clip_grad_workspace_bytes(count))

@@ -22,7 +22,7 @@
 
 namespace lmce {
 
-constexpr int AN_MAX_WARPS = 32;
+constexpr int AN_MAX_WARPS = 16;
 
 struct AddNormParams {
   const uint4* x;
@@ -53,24 +53,27 @@ struct AddNormBwdParams {
   float inv_cols;
 };
 
-// Sum (or maximum) over the threads of a row; `red` holds one value per warp of the block.
-// Every thread of the block calls it (the row groups run in step). Two __syncthreads: one
-// before the values are read, one (at the next call's start) before they are replaced.
+// Sum over the threads of a row, and with MAX the maximum of a second value in the same pass.
+// `red` holds one pair per warp of the block. Every thread of the block calls it (the row groups
+// run in step); the first __syncthreads keeps the last call's readers ahead of this one's writes.
 template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float* red, int warps) {
+__device__ __forceinline__ float2 row_reduce(float sum, float top, float2* red, int warps) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, t) : v + t;
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if constexpr (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
-  if (warps == 1) return v;
+  if (warps == 1) return make_float2(sum, top);
   const int w = threadIdx.x / 32;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[w] = v;
+  if ((threadIdx.x & 31) == 0) red[w] = make_float2(sum, top);
   __syncthreads();
   const int w0 = w / warps * warps;
-  float t = red[w0];
-  for (int i = 1; i < warps; ++i) t = MAX ? fmaxf(t, red[w0 + i]) : t + red[w0 + i];
+  float2 t = red[w0];
+  for (int i = 1; i < warps; ++i) {
+    t.x += red[w0 + i].x;
+    if constexpr (MAX) t.y = fmaxf(t.y, red[w0 + i].y);
+  }
   return t;
 }
 
@@ -84,7 +87,7 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* f) {
 
 template <bool BF16, int VPT, bool E4M3>
 __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
-  __shared__ float red[AN_MAX_WARPS];
+  __shared__ float2 red[AN_MAX_WARPS];
   const int g = threadIdx.x / p.threads, t = threadIdx.x - g * p.threads;
   const int warps = p.threads / 32;
   for (long long row0 = static_cast<long long>(blockIdx.x) * p.rows; row0 < p.n;
@@ -93,7 +96,7 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
     const bool live = row < p.n;
     float f[VPT][8];
     uint4 a[VPT], b[VPT];
-    float ss = 0.f;
+    float ss = 0.f, top = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * p.threads;
@@ -118,38 +121,48 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(f[i][j], f[i][j], ss);
-      }
-    }
-    const float rstd = rsqrtf(row_reduce<false>(ss, red, warps) * p.inv_cols + p.eps);
-    if (p.rstd && live && t == 0) p.rstd[row] = rstd;
-    float top = 0.f;
+        if constexpr (E4M3) {
+          float w[8];
+          unpack8<BF16>(__ldg(p.w + c), w);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * p.threads;
-      if (live && c < p.vec) {
-        float w[8];
-        unpack8<BF16>(__ldg(p.w + c), w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[i][j] = f[i][j] * rstd * w[j];
-          if constexpr (E4M3) top = fmaxf(top, fabsf(f[i][j]));
+          for (int j = 0; j < 8; ++j) {
+            f[i][j] *= w[j];
+            top = fmaxf(top, fabsf(f[i][j]));
+          }
         }
-        if constexpr (!E4M3) p.y[row * p.vec + c] = pack8<BF16>(f[i]);
       }
     }
-    if constexpr (E4M3) {
-      top = row_reduce<true>(top, red, warps);
-      // 448 is e4m3's largest value; a row of zeros (or one so small that the quotient
-      // vanishes) keeps scale 1
-      float scale = top / 448.0f;
-      if (!(scale > 0.f)) scale = 1.0f;
-      if (live && t == 0) p.scale[row] = scale;
+    const float2 both = row_reduce<E4M3>(ss, top, red, warps);
+    const float rstd = rsqrtf(both.x * p.inv_cols + p.eps);
+    if constexpr (!E4M3) {
+      if (p.rstd && live && t == 0) p.rstd[row] = rstd;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = t + i * p.threads;
+        if (live && c < p.vec) {
+          float w[8];
+          unpack8<BF16>(__ldg(p.w + c), w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * rstd * w[j];
+          p.y[row * p.vec + c] = pack8<BF16>(f[i]);
+        }
+      }
+    } else {
+      // rstd scales the whole row, so it cancels in q: with m = max|s w|, q = s w (448 / m), and
+      // only the scale, m rstd / 448, carries it. A row of zeros keeps scale 1, and so does one
+      // whose sum of squares is infinite (rstd = 0: its finite values become 0, as in y); a row
+      // with a NaN has rstd and scale NaN.
+      const float m = both.y;
+      const bool null = m == 0.f || rstd == 0.f;
+      const float k = null ? 0.f : 448.0f / m;
+      const bool tiny = !null && m < 1e-30f;  // 448 / m may be infinite
+      if (live && t == 0) p.scale[row] = null ? 1.0f : m * rstd / 448.0f;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = t + i * p.threads;
         if (live && c < p.vec) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] / scale;
+          for (int j = 0; j < 8; ++j) f[i][j] = tiny ? f[i][j] / m * 448.0f : f[i][j] * k;
           p.q[row * p.vec + c] = pack8_e4m3(f[i]);
         }
       }
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
 template <bool BF16, int VPT>
 __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const AddNormBwdParams p) {
   extern __shared__ float dw_smem[];  // [rows][8 * vec] when rows > 1 and dw is wanted
-  __shared__ float red[AN_MAX_WARPS];
+  __shared__ float2 red[AN_MAX_WARPS];
   const int g = threadIdx.x / p.threads, t = threadIdx.x - g * p.threads;
   const int warps = p.threads / 32;
   float acc[VPT][8];
@@ -172,52 +185,67 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const AddNormBwdParam
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * p.rows; row0 < p.n;
-       row0 += static_cast<long long>(gridDim.x) * p.rows) {
-    const long long row = row0 + g;
+  const long long stride = static_cast<long long>(gridDim.x) * p.rows;
+  uint4 na[VPT], nb[VPT], ne[VPT];
+  float nrstd = 0.f;
+  const auto load = [&](long long row) {
     const bool live = row < p.n;
-    uint4 a[VPT], b[VPT], e[VPT];
-    const float rstd = live ? p.rstd[row] : 0.f;
+    nrstd = live ? p.rstd[row] : 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * p.threads;
-      a[i] = b[i] = e[i] = make_uint4(0u, 0u, 0u, 0u);
+      na[i] = nb[i] = ne[i] = make_uint4(0u, 0u, 0u, 0u);
       if (live && c < p.vec) {
-        a[i] = __ldcs(p.s + row * p.vec + c);
-        if (p.dy) b[i] = __ldcs(p.dy + row * p.vec + c);
-        if (p.ds) e[i] = __ldcs(p.ds + row * p.vec + c);
+        na[i] = __ldcs(p.s + row * p.vec + c);
+        if (p.dy) nb[i] = __ldcs(p.dy + row * p.vec + c);
+        if (p.ds) ne[i] = __ldcs(p.ds + row * p.vec + c);
       }
     }
+  };
+  load(static_cast<long long>(blockIdx.x) * p.rows + g);
+  for (long long row0 = static_cast<long long>(blockIdx.x) * p.rows; row0 < p.n; row0 += stride) {
+    const long long row = row0 + g;
+    const bool live = row < p.n;
+    uint4 a[VPT], b[VPT], e[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      a[i] = na[i];
+      b[i] = nb[i];
+      e[i] = ne[i];
+    }
+    const float rstd = nrstd;
+    load(row + stride);  // in flight while this row is reduced
     float dot = 0.f;
-    float nrm[VPT][8], pw[VPT][8];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * p.threads;
       if (c < p.vec) {
-        float w[8];
-        unpack8<BF16>(a[i], nrm[i]);
-        unpack8<BF16>(b[i], pw[i]);
+        float s[8], d[8], w[8];
+        unpack8<BF16>(a[i], s);
+        unpack8<BF16>(b[i], d);
         unpack8<BF16>(__ldg(p.w + c), w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          nrm[i][j] *= rstd;
-          acc[i][j] = fmaf(pw[i][j], nrm[i][j], acc[i][j]);
-          pw[i][j] *= w[j];
-          dot = fmaf(pw[i][j], nrm[i][j], dot);
+          const float dn = d[j] * (s[j] * rstd);
+          acc[i][j] += dn;
+          dot = fmaf(dn, w[j], dot);
         }
       }
     }
     if (p.dx == nullptr) continue;
-    const float mean = row_reduce<false>(dot, red, warps) * p.inv_cols;
+    const float mean = row_reduce<false>(dot, 0.f, red, warps).x * p.inv_cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * p.threads;
       if (live && c < p.vec) {
-        float d[8];
-        unpack8<BF16>(e[i], d);
+        float s[8], d[8], w[8], o[8];
+        unpack8<BF16>(a[i], s);
+        unpack8<BF16>(b[i], d);
+        unpack8<BF16>(e[i], o);
+        unpack8<BF16>(__ldg(p.w + c), w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = fmaf(rstd, fmaf(-nrm[i][j], mean, pw[i][j]), d[j]);
-        p.dx[row * p.vec + c] = pack8<BF16>(d);
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(rstd, fmaf(d[j], w[j], -(s[j] * rstd) * mean), o[j]);
+        p.dx[row * p.vec + c] = pack8<BF16>(o);
       }
     }
   }
@@ -258,25 +286,22 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const AddNormBwdParam
   }
 }
 
-// dw[c] = dtype(sum over parts of dw_part[.][c]): 32 columns per block, 32 rows of threads
-// that each sum every 32nd part, then a fixed-order sum of the 32.
+// dw[c] = dtype(sum over parts of dw_part[.][c]): 8 columns per block (one 32-byte sector of a
+// part), 32 slices of threads that each sum every 32nd part, then a fixed-order sum of the 32.
 template <bool BF16>
-__global__ void __launch_bounds__(1024) add_norm_dw_kernel(const float* __restrict__ part, int parts, int cols,
-                                                           uint16_t* __restrict__ dw) {
-  __shared__ float sm[32][33];
-  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + cx;
+__global__ void __launch_bounds__(256) add_norm_dw_kernel(const float* __restrict__ part, int parts, int cols,
+                                                          uint16_t* __restrict__ dw) {
+  __shared__ float sm[8][33];
+  const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3;
+  const float* col = part + blockIdx.x * 8 + cx;  // cols is a multiple of 8
   float v = 0.f;
-  if (c < cols)
-    for (int r = ry; r < parts; r += 32) v += part[static_cast<size_t>(r) * cols + c];
-  sm[ry][cx] = v;
+#pragma unroll 4
+  for (int r = ry; r < parts; r += 32) v += col[static_cast<size_t>(r) * cols];
+  sm[cx][ry] = v;
   __syncthreads();
-  v = warp_sum(sm[cx][ry]);  // warp ry sums column ry over the 32 slices
-  const int co = blockIdx.x * 32 + ry;
-  if (cx == 0 && co < cols) {
-    const uint32_t u = pack2<BF16>(v, 0.f);
-    dw[co] = static_cast<uint16_t>(u & 0xffffu);
-  }
+  const int w = threadIdx.x / 32;
+  v = warp_sum(sm[w][threadIdx.x & 31]);
+  if ((threadIdx.x & 31) == 0) dw[blockIdx.x * 8 + w] = static_cast<uint16_t>(pack2<BF16>(v, 0.f) & 0xffffu);
 }
 
 }  // namespace lmce

@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kAnThreads = 512;      // most threads of a row
 constexpr int kAnBlock = 256;        // threads a block is filled up to with rows
-constexpr int kAnBwdBlocks = 592;    // partial rows of dw: four blocks on each of 148 SMs
+constexpr int kAnBwdBlocks = 296;    // partial rows of dw: the two blocks that 148 SMs hold at once
 constexpr int64_t kAnMaxHidden = 16384;
 
 struct RowShape {
@@ -104,37 +104,33 @@ int add_norm(const void* x, const void* residual, const void* weight, float eps,
 
 // -------------------------------------------------------- gradient clipping ---
 
-constexpr int kGnBlocks = 1184;  // eight blocks on each of 148 SMs; partial sums per launch
+constexpr int kGnBlocks = 592;  // the four blocks that 148 SMs hold at once; partial sums per launch
 
-template <int MAXT>
-int64_t fill_batch(GradBatch<MAXT>* b, void* const* grads, const int64_t* numels, const int32_t* dtypes,
-                   int64_t count) {
-  int64_t pieces = 0;
-  b->count = static_cast<int>(count);
-  for (int64_t i = 0; i < count; ++i) {
-    b->first[i] = static_cast<int>(pieces);
-    b->ptr[i] = grads[i];
-    b->numel[i] = numels[i];
-    b->dtype[i] = static_cast<uint8_t>(dtypes[i]);
-    const int64_t size = dtypes[i] == LMCE_DTYPE_F32 ? 4 : 2;
-    const int64_t bytes = (reinterpret_cast<uintptr_t>(grads[i]) & 15) + numels[i] * size;
-    pieces += (bytes + 16ll * GN_PIECE - 1) / (16ll * GN_PIECE);
-  }
-  b->first[count] = static_cast<int>(pieces);
-  return pieces;
+int64_t grad_pieces(const void* grad, int64_t numel, int32_t dtype) {
+  const int64_t size = dtype == LMCE_DTYPE_F32 ? 4 : 2;
+  const int64_t bytes = static_cast<int64_t>(reinterpret_cast<uintptr_t>(grad) & 15) + numel * size;
+  return numel > 0 ? (bytes + 16ll * GN_PIECE - 1) / (16ll * GN_PIECE) : 0;
 }
 
+// One launch of either pass over `count` tensors.
 template <int MAXT>
-int launch_clip(bool scale, void* const* grads, const int64_t* numels, const int32_t* dtypes, int64_t count,
+int launch_clip(bool scale, void* const* grads, const int64_t* numels, const int32_t* dtypes, int64_t count, int grid,
                 double* partial, int parts, float max_norm, float* total, cudaStream_t st) {
   GradBatch<MAXT> b;
-  const int64_t pieces = fill_batch(&b, grads, numels, dtypes, count);
-  if (scale) {
-    const int grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(pieces, 1), kGnBlocks));
-    grad_scale_kernel<MAXT><<<grid, GN_THREADS, 0, st>>>(b, partial, parts, max_norm, total);
-  } else {
-    grad_norm_kernel<MAXT><<<kGnBlocks, GN_THREADS, 0, st>>>(b, partial);
+  int64_t pieces = 0;
+  b.count = static_cast<int>(count);
+  for (int64_t i = 0; i < count; ++i) {
+    b.first[i] = static_cast<int>(pieces);
+    b.ptr[i] = grads[i];
+    b.numel[i] = numels[i];
+    b.dtype[i] = static_cast<uint8_t>(dtypes[i]);
+    pieces += grad_pieces(grads[i], numels[i], dtypes[i]);
   }
+  b.first[count] = static_cast<int>(pieces);
+  if (scale)
+    grad_scale_kernel<MAXT><<<(grid + 1) / 2, GN_THREADS, 0, st>>>(b, partial, parts, max_norm, total);
+  else
+    grad_norm_kernel<MAXT><<<grid, GN_THREADS, 0, st>>>(b, partial);
   return launched();
 }
 
@@ -320,10 +316,10 @@ int lmce_add_rmsnorm_backward(const void* d_y, const void* d_s, const void* s, c
   if (!d_weight) return LMCE_OK;
   const int cols = static_cast<int>(hidden_dim);
   if (dtype == LMCE_DTYPE_BF16)
-    add_norm_dw_kernel<true><<<(cols + 31) / 32, 1024, 0, st>>>(p.dw_part, grid, cols,
+    add_norm_dw_kernel<true><<<cols / 8, 256, 0, st>>>(p.dw_part, grid, cols,
                                                                 static_cast<uint16_t*>(d_weight));
   else
-    add_norm_dw_kernel<false><<<(cols + 31) / 32, 1024, 0, st>>>(p.dw_part, grid, cols,
+    add_norm_dw_kernel<false><<<cols / 8, 256, 0, st>>>(p.dw_part, grid, cols,
                                                                  static_cast<uint16_t*>(d_weight));
   return launched();
 }
@@ -353,7 +349,7 @@ int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t
       rc = fail(LMCE_ERR_UNSUPPORTED, "gradient %lld: dtype %d", (long long)i, dtypes[i]);
     const uintptr_t size = dtypes[i] == LMCE_DTYPE_F32 ? 4 : 2;
     const uintptr_t a = reinterpret_cast<uintptr_t>(grads[i]);
-    if (numels[i] < 0 || numels[i] > (1ll << 42) || (numels[i] > 0 && (a == 0 || a % size != 0)))
+    if (numels[i] < 0 || numels[i] > (1ll << 34) || (numels[i] > 0 && (a == 0 || a % size != 0)))
       rc = fail(LMCE_ERR_INVALID_ARGUMENT, "gradient %lld: null, misaligned or bad size", (long long)i);
     if (numels[i] > 0) r[used++] = {a, a + static_cast<uintptr_t>(numels[i]) * size};
   }
@@ -370,17 +366,24 @@ int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
   const int64_t batches = (count + GN_MAX_TENSORS - 1) / GN_MAX_TENSORS;
-  const int parts = static_cast<int>(batches) * kGnBlocks;
+  const auto grid_of = [&](int64_t i0, int64_t m) {
+    int64_t pieces = 0;
+    for (int64_t i = i0; i < i0 + m; ++i) pieces += grad_pieces(grads[i], numels[i], dtypes[i]);
+    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(pieces, 1), kGnBlocks));
+  };
+  int parts = 0;  // blocks of the first pass so far
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t k = 0; k < batches; ++k) {
       const int64_t b = pass == 0 ? k : batches - 1 - k;  // the scaling pass runs backwards
       const int64_t i0 = b * GN_MAX_TENSORS, m = std::min<int64_t>(count - i0, GN_MAX_TENSORS);
-      double* part = pass == 0 ? partial + b * kGnBlocks : partial;
+      const int grid = grid_of(i0, m);
+      double* part = pass == 0 ? partial + parts : partial;
+      if (pass == 0) parts += grid;
       float* total = b == 0 ? total_norm : nullptr;
       // the parameters of a launch with few tensors stay small
-      rc = m <= 64 ? launch_clip<64>(pass == 1, grads + i0, numels + i0, dtypes + i0, m, part, parts, max_norm, total,
-                                     st)
-                   : launch_clip<GN_MAX_TENSORS>(pass == 1, grads + i0, numels + i0, dtypes + i0, m, part, parts,
+      rc = m <= 64 ? launch_clip<64>(pass == 1, grads + i0, numels + i0, dtypes + i0, m, grid, part, parts, max_norm,
+                                     total, st)
+                   : launch_clip<GN_MAX_TENSORS>(pass == 1, grads + i0, numels + i0, dtypes + i0, m, grid, part, parts,
                                                  max_norm, total, st);
       if (rc) return rc;
     }
