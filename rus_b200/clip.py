@@ -68,9 +68,9 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     table = array("q", ptrs + list(map(torch.Tensor.numel, grads)))
     codes = array("i", map(_GRAD_DTYPES.__getitem__, kinds))
     at = table.buffer_info()[0]
-    total = torch.empty((), dtype=torch.float32, device=dev)
+    total = grads[0].new_empty((), dtype=torch.float32)
     ws_bytes = int(_lib.load().lmce_clip_grad_workspace_bytes(count))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = total.new_empty(ws_bytes, dtype=torch.uint8)
 
     def run(limit):
         _lib.launch(dev, "lmce_clip_grad_norm", at, at + 8 * count, codes.buffer_info()[0], count, limit,

@@ -154,15 +154,21 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
       // with a NaN has rstd and scale NaN.
       const float m = both.y;
       const bool null = m == 0.f || rstd == 0.f;
-      const float k = null ? 0.f : 448.0f / m;
-      const bool tiny = !null && m < 1e-30f;  // 448 / m may be infinite
+      float k = null ? 0.f : 448.0f / m;
+      if (!null && m < 1e-30f) {  // 448 / m may be infinite
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] *= 0x1p100f;
+        k = 448.0f / (m * 0x1p100f);
+      }
       if (live && t == 0) p.scale[row] = null ? 1.0f : m * rstd / 448.0f;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = t + i * p.threads;
         if (live && c < p.vec) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[i][j] = tiny ? f[i][j] / m * 448.0f : f[i][j] * k;
+          for (int j = 0; j < 8; ++j) f[i][j] *= k;
           p.q[row * p.vec + c] = pack8_e4m3(f[i]);
         }
       }

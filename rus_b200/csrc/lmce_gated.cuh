@@ -686,28 +686,27 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 
 // --------------------------------------------------- backward: dg and du ---
 
-// One warp per 32 tokens x 32 features of the saved blocks, 16 features at a time: g and u
-// arrive as they were stored (512 contiguous bytes per load), dh and the results pass through a
-// 48-byte-pitch row staging (conflict-free for 16-byte accesses by row and by column pair).
-// Memory-bound, 14 bytes per element: halves of 16 features keep a thread under 64 registers, so
-// that 32 warps per SM cover each other's loads.
-constexpr int GATED_DACT_WARPS = 4;
+// A block of four warps per 32 tokens x 64 features (two of the saved blocks), 16 features per
+// warp and one token per lane: g and u arrive as they were stored (512 contiguous bytes per
+// load); dh and the results pass through shared memory, 128 contiguous bytes per token in global
+// memory and a 144-byte pitch here (conflict-free by row and by column). Memory-bound, 14 bytes
+// per element. 16 features keep a thread within 64 registers, so that 32 warps per SM cover each
+// other's loads.
+constexpr int GATED_DACT_THREADS = 128;
 template <bool BF16>
-__global__ void __launch_bounds__(32 * GATED_DACT_WARPS, 8)
+__global__ void __launch_bounds__(GATED_DACT_THREADS, 8)
     gated_dact_kernel(const float4* __restrict__ saved, const uint4* __restrict__ dh, int n, int f, int act,
                       uint4* __restrict__ dg, uint4* __restrict__ du) {
-  __shared__ uint4 st[GATED_DACT_WARPS][32][3];
+  __shared__ uint4 st[2][32][9];  // dh, then dg; du
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int fb = f / 32, vec = f / 8;
-  const long long halves = static_cast<long long>((n + 31) / 32) * fb * 2;
-  const int r0 = lane >> 1, c = lane & 1;
-  for (long long b = static_cast<long long>(blockIdx.x) * GATED_DACT_WARPS + warp; b < halves;
-       b += static_cast<long long>(gridDim.x) * GATED_DACT_WARPS) {
-    const long long blk = b >> 1;
-    const int h = static_cast<int>(b & 1);
-    const int rb = static_cast<int>(blk / fb), cb = static_cast<int>(blk - static_cast<long long>(rb) * fb);
-    const float4* sv = saved + blk * (2 * GATED_SAVE_BLOCK / 4) + h * 128 + lane;
-    const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 4 + h * 2 + c;
+  const int tf = f / 64, vec = f / 8;
+  const long long tiles = static_cast<long long>((n + 31) / 32) * tf;
+  const int r0 = threadIdx.x >> 3, c = threadIdx.x & 7;  // global accesses: rows r0 and r0 + 16
+  for (long long b = blockIdx.x; b < tiles; b += gridDim.x) {
+    const int rb = static_cast<int>(b / tf), cb = static_cast<int>(b - static_cast<long long>(rb) * tf);
+    const float4* sv = saved + (static_cast<long long>(rb) * (f / 32) + cb * 2 + (warp >> 1)) * (2 * GATED_SAVE_BLOCK / 4) +
+                       (warp & 1) * 128 + lane;
+    const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 8 + c;
     const bool live0 = rb * 32 + r0 < n, live1 = rb * 32 + r0 + 16 < n;
     float4 g[4], u[4];
     uint4 d0 = make_uint4(0u, 0u, 0u, 0u), d1 = d0;
@@ -717,13 +716,14 @@ __global__ void __launch_bounds__(32 * GATED_DACT_WARPS, 8)
     for (int j = 0; j < 4; ++j) g[j] = __ldcs(sv + j * 32);
 #pragma unroll
     for (int j = 0; j < 4; ++j) u[j] = __ldcs(sv + 256 + j * 32);
-    __syncwarp();  // the last rows have left the staging
-    st[warp][r0][c] = d0;
-    st[warp][r0 + 16][c] = d1;
-    __syncwarp();
+    st[0][r0][c] = d0;
+    st[0][r0 + 16][c] = d1;
+    __syncthreads();
     float d[16], e[16];
-    unpack8<BF16>(st[warp][lane][0], d);
-    unpack8<BF16>(st[warp][lane][1], d + 8);
+    uint4* own0 = &st[0][lane][warp * 2];
+    uint4* own1 = &st[1][lane][warp * 2];
+    unpack8<BF16>(own0[0], d);
+    unpack8<BF16>(own0[1], d + 8);
     const float* gf = reinterpret_cast<const float*>(g);
     const float* uf = reinterpret_cast<const float*>(u);
 #pragma unroll
@@ -733,16 +733,20 @@ __global__ void __launch_bounds__(32 * GATED_DACT_WARPS, 8)
       e[j] = d[j] * a;
       d[j] = d[j] * uf[j] * da;
     }
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      __syncwarp();
-      st[warp][lane][0] = pack8<BF16>(pass ? e : d);
-      st[warp][lane][1] = pack8<BF16>((pass ? e : d) + 8);
-      __syncwarp();
-      uint4* out = pass ? du : dg;
-      if (live0) out[at] = st[warp][r0][c];
-      if (live1) out[at + 16ll * vec] = st[warp][r0 + 16][c];
+    own0[0] = pack8<BF16>(d);
+    own0[1] = pack8<BF16>(d + 8);
+    own1[0] = pack8<BF16>(e);
+    own1[1] = pack8<BF16>(e + 8);
+    __syncthreads();
+    if (live0) {
+      dg[at] = st[0][r0][c];
+      du[at] = st[1][r0][c];
     }
+    if (live1) {
+      dg[at + 16ll * vec] = st[0][r0 + 16][c];
+      du[at + 16ll * vec] = st[1][r0 + 16][c];
+    }
+    __syncthreads();
   }
 }
 

@@ -497,15 +497,13 @@ int lmce_gated_backward(const void* d_h, const void* saved, const void* x, const
   const int64_t n = n_rows, h = hidden_dim, f = ffn_dim;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
-  const int64_t halves = (n + 31) / 32 * (f / 16);
-  const int dgrid = static_cast<int>(
-      std::min<int64_t>((halves + GATED_DACT_WARPS - 1) / GATED_DACT_WARPS, d->sms * 8ll));
+  const int dgrid = static_cast<int>(std::min<int64_t>((n + 31) / 32 * (f / 64), d->sms * 8ll));
   if (bf16)
-    gated_dact_kernel<true><<<dgrid, 32 * GATED_DACT_WARPS, 0, st>>>(
+    gated_dact_kernel<true><<<dgrid, GATED_DACT_THREADS, 0, st>>>(
         static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
         act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
   else
-    gated_dact_kernel<false><<<dgrid, 32 * GATED_DACT_WARPS, 0, st>>>(
+    gated_dact_kernel<false><<<dgrid, GATED_DACT_THREADS, 0, st>>>(
         static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
         act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
   if (int rc = launched()) return rc;

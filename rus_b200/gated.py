@@ -44,11 +44,11 @@ def _forward(x, w_gate, w_up, activation, save: bool):
     f, h = w_gate.shape
     xc, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
     n = xc.numel() // h
-    out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=x.device)
+    out = xc.new_empty((*x.shape[:-1], f))
     saved = None
     if n > 0:
         if save:
-            saved = torch.empty(int(_lib.load().lmce_gated_saved_bytes(n, f)), dtype=torch.uint8, device=x.device)
+            saved = xc.new_empty(int(_lib.load().lmce_gated_saved_bytes(n, f)), dtype=torch.uint8)
         _lib.launch(x.device, "lmce_gated_linear", xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), n, h, f,
                     _DTYPES[x.dtype], ACTIVATIONS[activation], out.data_ptr(), _ptr(saved))
     return out, xc, wg, wu, saved
@@ -77,7 +77,7 @@ class GatedLinearFn(torch.autograd.Function):
         if n > 0:
             g = _rows(dh)
             ws_bytes = int(_lib.load().lmce_gated_bwd_workspace_bytes(n, h, f, want_x, want_g + want_u))
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws = x.new_empty(ws_bytes, dtype=torch.uint8)
             _lib.launch(dev, "lmce_gated_backward", g.data_ptr(), saved.data_ptr(), x.data_ptr(), wg.data_ptr(),
                         wu.data_ptr(), n, h, f, _DTYPES[x.dtype], ACTIVATIONS[ctx.activation], _ptr(dx), _ptr(dg),
                         _ptr(du), ws.data_ptr(), ws_bytes)
@@ -133,7 +133,7 @@ def gated_linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w_gate: torch.Tens
     xc, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
     sx, sg, su = _rows(x_scale), _rows(gate_scale), _rows(up_scale)
     n = xc.numel() // h
-    out = torch.empty((*x.shape[:-1], f), dtype=out_dtype, device=x.device)
+    out = xc.new_empty((*x.shape[:-1], f), dtype=out_dtype)
     if n > 0:
         _lib.launch(x.device, "lmce_gated_linear_e4m3", xc.data_ptr(), sx.data_ptr(), wg.data_ptr(), sg.data_ptr(),
                     wu.data_ptr(), su.data_ptr(), n, h, f, _DTYPES[out_dtype], ACTIVATIONS[activation],

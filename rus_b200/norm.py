@@ -56,7 +56,7 @@ def _forward(x, residual, weight, eps, keep_rstd: bool):
     n = xc.numel() // h
     y = torch.empty_like(xc)
     s = xc if rc is None else torch.empty_like(xc)
-    rstd = torch.empty(n, dtype=torch.float32, device=x.device) if keep_rstd else None
+    rstd = xc.new_empty(n, dtype=torch.float32) if keep_rstd else None
     if n > 0:
         _lib.launch(x.device, "lmce_add_rmsnorm", xc.data_ptr(), _ptr(rc), w.data_ptr(), eps, n, h, _DTYPES[x.dtype],
                     s.data_ptr(), y.data_ptr(), _ptr(rstd))
@@ -91,7 +91,7 @@ class AddRMSNormFn(torch.autograd.Function):
             ws, ws_bytes = None, 0
             if want_dw:
                 ws_bytes = int(_lib.load().lmce_add_rmsnorm_bwd_workspace_bytes(n, h))
-                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+                ws = s.new_empty(ws_bytes, dtype=torch.uint8)
             _lib.launch(dev, "lmce_add_rmsnorm_backward", _ptr(g), _ptr(gs), s.data_ptr(), w.data_ptr(),
                         rstd.data_ptr(), n, h, _DTYPES[s.dtype], _ptr(dx), dw.data_ptr() if want_dw else None,
                         _ptr(ws), ws_bytes)
@@ -132,8 +132,8 @@ def add_rms_norm_e4m3(x: torch.Tensor, residual: torch.Tensor | None, weight: to
     xc, w = _rows(x), _rows(weight)
     rc = None if residual is None else _rows(residual)
     n = xc.numel() // h
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = torch.empty_like(xc, dtype=torch.float8_e4m3fn)
+    scale = xc.new_empty(x.shape[:-1], dtype=torch.float32)
     s = xc if rc is None else torch.empty_like(xc)
     if n > 0:
         _lib.launch(x.device, "lmce_add_rmsnorm_e4m3", xc.data_ptr(), _ptr(rc), w.data_ptr(), eps, n, h,

@@ -139,6 +139,19 @@ def test_e4m3(cuda_device, n, h, dtype):
     assert (q.float().abs().amax(-1)[live] == 448).all()
 
 
+@pytest.mark.parametrize("size", [1e-38, 1e-34, 1e-31, 1e-25, 1e15])
+def test_e4m3_of_rows_of_any_size(cuda_device, size):
+    x, r, w, dy, ds = _inputs(cuda_device, 4, 520, torch.bfloat16, seed=9)
+    r = (r.float() * size).bfloat16()
+    q, scale, s = add_rms_norm_e4m3(r, None, w, 1e-6)
+    y_ref = _reference(s, w, dy, ds, 1e-6)[0]
+    top = y_ref.abs().amax(-1) / 448
+    # values of 1e-38 are under the smallest normal fp32, 2^-126, in parts: steps of 2^-149
+    _close(scale, top, top * 2 ** -20 + 2.0 ** -146 * 1e3 / 448)
+    _close(q.double() * scale.double()[:, None], y_ref,
+           y_ref.abs() * (2 ** -4 + 2 ** -18) + top[:, None] * 2 ** -10 + 2.0 ** -145 * 1e3)
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 def test_bad_values_stay_in_their_row(cuda_device, value):
     x, r, w, dy, ds = _inputs(cuda_device, 9, 896, torch.bfloat16, seed=6)
