@@ -26,7 +26,9 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
 
     ``parameters`` is a tensor or an iterable of tensors; those without a gradient are
     skipped, one that is listed twice counts once. Gradients: fp16, bf16 or fp32, mixed, on
-    one CUDA device, of any alignment (a non-contiguous one goes through a copy). They are
+    one CUDA device, of any alignment (a non-contiguous one goes through a copy), none
+    overlapping another in memory. The norm is over this process's gradients: for a
+    vocabulary shard it covers the shard. They are
     multiplied by ``max_norm / (norm + 1e-6)`` where that is below 1 and left as they are
     otherwise; a norm that is not a number makes them all so, an infinite one zeroes the
     finite ones, as in torch; ``max_norm=inf`` only measures. Nothing is read back to the host
@@ -61,6 +63,9 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     if not all(map(torch.Tensor.is_contiguous, grads)):
         for i, g in enumerate(grads):
             if not g.is_contiguous():
+                if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                    raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT,
+                                         "clip_grad_norm_: an expanded gradient (its elements share memory)")
                 c = g.contiguous()
                 copies.append((g, c))
                 ptrs[i] = c.data_ptr()
