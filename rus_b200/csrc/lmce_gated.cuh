@@ -73,7 +73,8 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) 
   const float om = e < 1e30f ? e * s : 1.0f;  // 1 - sig, without its cancellation
   const float dv = act == ACT_SILU ? 1.0f : 1.5957691216057308f * fmaf(0.134145f * g, g, 1.0f);
   a = g * s;
-  da = fmaf(a * om, dv, s);
+  const float t = a * om;
+  da = t == 0.f ? s : fmaf(t, dv, s);  // far out sig or 1 - sig is 0 and v' may be infinite
 }
 
 // ------------------------------------------------------------ few tokens ---

@@ -208,6 +208,21 @@ def test_far_arguments(cuda_device, kind):
     _assert_within(grads[0][:, 0], dx0, dx0.abs() * 2.1 * _eps(torch.bfloat16) + 1e-6)
 
 
+@pytest.mark.parametrize("kind", ["silu", "gelu_tanh"])
+def test_arguments_whose_squares_overflow(cuda_device, kind):
+    x = torch.zeros(4, 64, device=cuda_device, dtype=torch.bfloat16)
+    x[:, 0] = torch.tensor([-1e30, -1e20, 1e20, 1e30], device=cuda_device)
+    x[:, 1] = 1.0
+    wg, wu = (torch.zeros(64, 64, device=cuda_device, dtype=torch.bfloat16) for _ in range(2))
+    wg[:, 0], wu[:, 1] = 1.0, 0.5
+    x.requires_grad_(True)
+    out = gated_linear(x, wg, wu, kind)
+    (dx,) = torch.autograd.grad(out, x, torch.ones_like(out))
+    want = (x.detach()[:, :1].double().clamp(min=0) * 0.5).expand(-1, 64)
+    _assert_within(out.detach(), want, want * _eps(torch.bfloat16) * 1.01)
+    assert torch.equal(dx[:, 0].float(), torch.tensor([0.0, 0.0, 32.0, 32.0], device=cuda_device))
+
+
 def test_strides_alignment_and_leading_dimensions(cuda_device):
     x, wg, wu, dh = _inputs(cuda_device, 150, 192, 320, torch.bfloat16, seed=7)
     leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu)]
