@@ -50,8 +50,9 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients on several devices")
     kinds = list(map(_dtype_of, grads))
     if not _GRAD_DTYPES.keys() >= set(kinds):
+        other = set(kinds) - _GRAD_DTYPES.keys()
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
-                             f"clip_grad_norm_: gradients of {set(kinds) - _GRAD_DTYPES.keys()} (need fp16, bf16, fp32)")
+                             f"clip_grad_norm_: gradients of {other} (need fp16, bf16 or fp32)")
     try:
         ptrs = list(map(torch.Tensor.data_ptr, grads))
     except RuntimeError as e:  # no storage

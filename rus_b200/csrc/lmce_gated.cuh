@@ -20,9 +20,11 @@
 // With training the epilogue also keeps g and u in fp32, in blocks of 32 tokens x 32 features
 // laid out as the accumulator is read ([g | u][8 column groups of 4][32 tokens][4]), so each
 // store instruction of a warp writes 512 contiguous bytes. fp32 because dg and du are rounded
-// once already: with 16-bit g and u the gradients' error grew from 1.4 to 1.8 times that of a
-// single rounding, and the bytes are those an eager block keeps for its backward (g, u, act(g)
-// and h at 2 bytes each).
+// once already: a gradient's error is sqrt(2) times that of its own rounding alone, and would be
+// 1.8 times with g and u in the inputs' type. The bytes are those an eager block keeps for its
+// backward (g, u, act(g) and h at 2 bytes each). The stores cost the forward 10% (8192 x 4096 x
+// 14336) to 45% (4096 x 896 x 4864), in proportion to their bytes and alike when all of them hit
+// L2: they share the SM's path with the operands.
 //
 // e4m3 operands (serving): the same kernel with kind::f8f6f4, K = 256 per stage in the same
 // bytes; g and u are scaled by the row's and the feature's scale in the epilogue.
@@ -705,8 +707,8 @@ __global__ void __launch_bounds__(GATED_DACT_THREADS, 8)
   const int r0 = threadIdx.x >> 3, c = threadIdx.x & 7;  // global accesses: rows r0 and r0 + 16
   for (long long b = blockIdx.x; b < tiles; b += gridDim.x) {
     const int rb = static_cast<int>(b / tf), cb = static_cast<int>(b - static_cast<long long>(rb) * tf);
-    const float4* sv = saved + (static_cast<long long>(rb) * (f / 32) + cb * 2 + (warp >> 1)) * (2 * GATED_SAVE_BLOCK / 4) +
-                       (warp & 1) * 128 + lane;
+    const long long blk = static_cast<long long>(rb) * (f / 32) + cb * 2 + (warp >> 1);
+    const float4* sv = saved + blk * (2 * GATED_SAVE_BLOCK / 4) + (warp & 1) * 128 + lane;
     const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 8 + c;
     const bool live0 = rb * 32 + r0 < n, live1 = rb * 32 + r0 + 16 < n;
     float4 g[4], u[4];
@@ -762,6 +764,8 @@ __global__ void __launch_bounds__(GATED_DACT_THREADS, 8)
 // DX units are the longer ones and come first; the pairs that get one DX unit less than the
 // others take that many stages' worth of DW units before the rest is dealt out in turn. The
 // assignment is a function of the sizes alone: no counters, the same sums every time.
+constexpr int GATED_UNIT_STAGES = 5;  // a unit's epilogue takes about as long as five stages
+
 struct GatedBwdParams {
   int N, H, F;
   int n_dx, splits, dx_stages;   // DX units (tiles x splits), splits per tile, K stages of a whole tile
@@ -784,8 +788,8 @@ struct GatedUnits {
     n_dw = p.n_dw;
     const int heavy = n_dx % pairs;
     const int light = heavy ? pairs - heavy : 0;
-    const int lx = p.splits > 0 ? p.dx_stages / p.splits : 0;
-    const int ld = max(1, (p.N + P_KB - 1) / P_KB);
+    const int lx = max(GATED_UNIT_STAGES, (p.dx_stages + p.splits - 1) / p.splits);
+    const int ld = max(GATED_UNIT_STAGES, (p.N + P_KB - 1) / P_KB);
     const int ahead = light ? lx / ld : 0;
     common = static_cast<int>(min(static_cast<long long>(n_dw), static_cast<long long>(light) * ahead));
     extra = pair >= heavy && light ? ahead : 0;

@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(GN_THREADS, 4) grad_norm_kernel(const __grid_c
 
 // Adds the partial sums (every block the same way), and scales this launch's tensors when the
 // norm exceeds max_norm. Two blocks per SM with 32 KB of loads each in flight: four (64
-// registers) write 10% slower (one B200, 988 MB: 315 against 350 us). `total`, if not null, receives the norm (block 0).
+// registers) write 10% slower (one B200, 988 MB: 315 against 350 us). `total`, if not null,
+// receives the norm (block 0).
 template <int MAXT>
 __global__ void __launch_bounds__(GN_THREADS, 2) grad_scale_kernel(const __grid_constant__ GradBatch<MAXT> b,
                                                                 const double* __restrict__ partial, int parts,

@@ -6,7 +6,8 @@ K * 2^-24 * sum |x w| in the worst case and a small multiple of sqrt(K) * 2^-24 
 such inputs; 2^-18 * |x| |w| (norms) is taken for K <= 4096, for g and u each, and 2^-18 of the
 values for the activation. Gradients contract dg and du rounded to the type, independent
 roundings: an element of dx is off by the norm of the terms' errors times some standard
-deviations; 6 norms are allowed, next to the result's own half step. e4m3 operands are exact inputs: the tolerance is the same as for h."""
+deviations; 6 norms are allowed, next to the result's own half step. e4m3 operands are exact
+inputs: the tolerance is the same as for h."""
 from __future__ import annotations
 
 import pytest

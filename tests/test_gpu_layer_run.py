@@ -154,7 +154,8 @@ def test_refusals_on_the_device(cuda_device):
         lambda: gated_linear(x, wg.cpu(), wg.cpu()), lambda: gated_linear(x[:, :64], wg, wg),
         lambda: gated_linear(x[:, :96], wg[:, :96], wg[:, :96]), lambda: gated_linear(x, wg[:32], wg[:32]),
         lambda: gated_linear(x.float(), wg.float(), wg.float()), lambda: gated_linear(x, wg, wg, "tanh"),
-        lambda: gated_linear_e4m3(x, sx, wg, sw, wg, sw), lambda: gated_linear_e4m3(f8(x), sx[:2], f8(wg), sw, f8(wg), sw),
+        lambda: gated_linear_e4m3(x, sx, wg, sw, wg, sw),
+        lambda: gated_linear_e4m3(f8(x), sx[:2], f8(wg), sw, f8(wg), sw),
         lambda: gated_linear_e4m3(f8(x), sx, f8(wg), sw[:8], f8(wg), sw),
         lambda: gated_linear_e4m3(f8(x), sx.half(), f8(wg), sw, f8(wg), sw),
         lambda: gated_linear_e4m3(f8(x[:, :64]), sx, f8(wg[:, :64]), sw, f8(wg[:, :64]), sw),
