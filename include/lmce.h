@@ -266,7 +266,7 @@ LMCE_API int lmce_embedding_lookup(const void* weight, const int64_t* token_ids,
 /* -------------------------------------------- residual add + RMSNorm */
 
 /* Residual addition with its RMSNorm, the front of a decoder block's sub-layer (the
- * reference fuses the pair in rms_norm_fwd, kernels.py:125-164):
+ * reference fuses the pair in rms_norm_fwd, kernels.py:124-164):
  *   s = dtype(x + residual),  rstd = 1/sqrt(mean(s^2) + eps),  y = dtype(s * rstd * weight)
  * with fp32 sums and one rounding of y. residual may be null: s = x, and s_out is not used.
  *   x, residual, s_out, y_out  [n_rows, hidden_dim] dtype, contiguous, 16-byte aligned
@@ -285,7 +285,7 @@ LMCE_API int lmce_add_rmsnorm_e4m3(const void* x, const void* residual, const vo
 
 LMCE_API size_t lmce_add_rmsnorm_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim);
 
-/* Backward of lmce_add_rmsnorm (reference: rms_norm_bwd, kernels.py:167-199, which has no
+/* Backward of lmce_add_rmsnorm (reference: rms_norm_bwd, kernels.py:167-190, which has no
  * weight gradient). s is s_out (or x without residual). d_y and d_s are the gradients of y and
  * s (each nullable: zero); d_x is the gradient of x and of residual alike (nullable);
  * d_weight [hidden_dim] dtype (nullable; the workspace is used only with it). Deterministic. */
@@ -298,7 +298,7 @@ LMCE_API int lmce_add_rmsnorm_backward(const void* d_y, const void* d_s, const v
 enum { LMCE_ACT_SILU = 0, LMCE_ACT_GELU_TANH = 1 };
 
 /* The gated projection of a feed-forward block in one kernel (the reference: two cuBLAS
- * products and swiglu_fwd, kernels.py:355-400):
+ * products and its SwiGLU kernels, kernels.py:355-446):
  *   h = act(x . w_gate^T) * (x . w_up^T),  fp32 accumulation and activation, one rounding
  *   x [n_rows, hidden_dim], w_gate and w_up [ffn_dim, hidden_dim], h_out [n_rows, ffn_dim]
  * dtype, contiguous, 16-byte aligned; hidden_dim and ffn_dim multiples of 64. `saved`
@@ -319,8 +319,8 @@ LMCE_API int lmce_gated_linear_e4m3(const void* x, const float* x_scale, const v
 LMCE_API size_t lmce_gated_bwd_workspace_bytes(int64_t n_rows, int64_t hidden_dim, int64_t ffn_dim, int want_dx,
                                                int n_weights);
 
-/* Backward of lmce_gated_linear (the reference: swiglu_bwd, kernels.py:403-446, and two cuBLAS
- * products; its weights are frozen):
+/* Backward of lmce_gated_linear (the reference's weights are frozen: its SwiGLU backward,
+ * kernels.py:355-446, and products for d_x):
  *   dg = dtype(d_h * u * act'(g)), du = dtype(d_h * act(g)),
  *   d_x = dg . w_gate + du . w_up, d_gate = dg^T . x, d_up = du^T . x
  * Each of d_x, d_gate and d_up may be null (not all). The workspace is 256-byte aligned,

@@ -1,6 +1,6 @@
 // Residual addition with its RMSNorm, forward (16-bit or e4m3 output) and backward: what a
 // decoder block runs in front of each of its projections (the reference fuses the same
-// pair in rms_norm_fwd / rms_norm_bwd, solution/kernels.py:125-199).
+// pair in rms_norm_fwd / rms_norm_bwd, solution/kernels.py:124-190).
 //   s = dtype(x + residual)            the residual stream, kept in the inputs' type
 //   rstd = 1 / sqrt(mean(s^2) + eps)   fp32
 //   y = dtype(s * rstd * w)            one rounding

@@ -2,7 +2,7 @@
 //   h = act(x . Wg^T) * (x . Wu^T)                  x [N, H], Wg and Wu [F, H], h [N, F]
 //   act(g) = g * sig(v): silu v = g; gelu (tanh form) v = 2 sqrt(2/pi) (g + 0.044715 g^3),
 //   which is 0.5 g (1 + tanh(v / 2)) without the cancellation of 1 + tanh
-// (the reference runs two cuBLAS products and the kernels swiglu_fwd / swiglu_bwd,
+// (the reference runs two cuBLAS products and its SwiGLU kernels,
 // solution/kernels.py:355-446, with g and u in memory between them).
 // Backward, from dh and the forward's g and u:
 //   dg = dh * u * act'(g),  du = dh * act(g)        rounded to the inputs' type (tensor-core operands)

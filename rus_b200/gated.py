@@ -1,7 +1,7 @@
 """Gated projection of a feed-forward block: both projections, the activation and the product
 in one kernel, with its backward; and the same on e4m3 operands for serving.
 
-The reference computes it as two cuBLAS products and ``swiglu_fwd`` / ``swiglu_bwd``
+The reference computes it as two cuBLAS products and its SwiGLU kernels
 (``solution/kernels.py:355-446``, ``FusedMLPGLUFn`` in ``solution/ops.py:57-85``) around
 frozen weights; here the weights get their gradients as well. The down projection that
 follows is one plain product. CUDA tensors only: there is no CPU path.

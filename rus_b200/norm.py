@@ -1,8 +1,8 @@
 """Residual addition with its RMSNorm, and the same with an e4m3 output for 8-bit products.
 
 What a decoder block runs in front of its attention and its feed-forward projections; the
-reference fuses the pair in ``rms_norm_fwd`` (``solution/kernels.py:125-164``) with the
-backward ``rms_norm_bwd`` (``kernels.py:167-199``, no weight gradient). ``rms_norm_pack``
+reference fuses the pair in ``rms_norm_fwd`` (``solution/kernels.py:124-164``) with the
+backward ``rms_norm_bwd`` (``kernels.py:167-190``, no weight gradient). ``rms_norm_pack``
 (``packing.py``) is the final norm in front of the head; these stand in front of every
 block. CUDA tensors only: there is no CPU path.
 """
