@@ -49,19 +49,23 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     if set(map(torch.Tensor.get_device, grads)) != {dev.index}:
         raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients on several devices")
     kinds = list(map(_dtype_of, grads))
-    if not _GRAD_DTYPES.keys() >= set(kinds):
-        other = set(kinds) - _GRAD_DTYPES.keys()
+    distinct = set(kinds)
+    if not _GRAD_DTYPES.keys() >= distinct:
+        other = distinct - _GRAD_DTYPES.keys()
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED,
                              f"clip_grad_norm_: gradients of {other} (need fp16, bf16 or fp32)")
     try:
-        ptrs = list(map(torch.Tensor.data_ptr, grads))
+        table = array("q", map(torch.Tensor.data_ptr, grads))
     except RuntimeError as e:  # no storage
         raise _lib.LmceError(_lib.LMCE_ERR_UNSUPPORTED, f"clip_grad_norm_: a gradient that is not dense ({e})") from e
-    if len(set(ptrs)) < len(ptrs):  # a parameter listed twice counts once (empty gradients share address 0)
-        grads = [g for p in dict.fromkeys(params) if (g := p.grad) is not None]
-        kinds, ptrs = list(map(_dtype_of, grads)), list(map(torch.Tensor.data_ptr, grads))
     copies = []
     if not all(map(torch.Tensor.is_contiguous, grads)):
+        # the copies hide from the library what shares memory
+        if len(set(map(id, params))) < len(params):
+            return clip_grad_norm_(dict.fromkeys(params), max_norm, error_if_nonfinite)
+        starts = [a for a, g in zip(table, grads) if g.numel() > 0]
+        if len(set(starts)) < len(starts):
+            raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients overlap in memory")
         for i, g in enumerate(grads):
             if not g.is_contiguous():
                 if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
@@ -69,10 +73,13 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
                                          "clip_grad_norm_: an expanded gradient (its elements share memory)")
                 c = g.contiguous()
                 copies.append((g, c))
-                ptrs[i] = c.data_ptr()
+                table[i] = c.data_ptr()
     count = len(grads)
-    table = array("q", ptrs + list(map(torch.Tensor.numel, grads)))
-    codes = array("i", map(_GRAD_DTYPES.__getitem__, kinds))
+    table.extend(map(torch.Tensor.numel, grads))
+    if len(distinct) == 1:
+        codes = array("i", [_GRAD_DTYPES[kinds[0]]]) * count
+    else:
+        codes = array("i", map(_GRAD_DTYPES.__getitem__, kinds))
     at = table.buffer_info()[0]
     total = grads[0].new_empty((), dtype=torch.float32)
     ws_bytes = int(_lib.load().lmce_clip_grad_workspace_bytes(count))
@@ -82,11 +89,17 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
         _lib.launch(dev, "lmce_clip_grad_norm", at, at + 8 * count, codes.buffer_info()[0], count, limit,
                     total.data_ptr(), ws.data_ptr(), ws_bytes)
 
-    if error_if_nonfinite:
-        run(float("inf"))  # measures only
-        if not torch.isfinite(total):
-            raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {total.item()}, nothing was scaled")
-    run(max_norm)
+    try:
+        if error_if_nonfinite:
+            run(float("inf"))  # measures only
+            if not torch.isfinite(total):
+                raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {total.item()}, nothing was scaled")
+        run(max_norm)
+    except _lib.LmceError as e:
+        # refused before any launch; a parameter listed twice counts once
+        if e.code == _lib.LMCE_ERR_INVALID_ARGUMENT and len(set(map(id, params))) < len(params):
+            return clip_grad_norm_(dict.fromkeys(params), max_norm, error_if_nonfinite)
+        raise
     for g, c in copies:
         g.copy_(c)
     return total

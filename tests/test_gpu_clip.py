@@ -130,6 +130,16 @@ def test_repeated_missing_and_strided(cuda_device):
     _check([p], 2.0)
     assert torch.equal(wide[:, 1::2], left)
     assert clip_grad_norm_([none], 1.0).item() == 0.0
+    before = p.grad.double().norm().item()  # the strided one listed twice, and with an empty one
+    empty = torch.zeros(0, device=cuda_device, requires_grad=True)
+    empty.grad = torch.zeros_like(empty)
+    total = clip_grad_norm_([p, empty, p, empty], 0.5, error_if_nonfinite=True)
+    assert abs(total.item() - before) <= before * 2 ** -20
+    assert abs(p.grad.double().norm().item() - 0.5) <= 0.5 * 2 ** -10
+    other = torch.zeros(40, 30, device=cuda_device, requires_grad=True)
+    other.grad = p.grad
+    with pytest.raises(_lib.LmceError, match="overlap"):
+        clip_grad_norm_([p, other], 0.1)
     total = clip_grad_norm_(params[1], 1e9)  # a single tensor
     assert total.item() > 0
 
