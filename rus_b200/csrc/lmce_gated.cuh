@@ -17,14 +17,16 @@
 // read is all that counts. Stages, loads (one 256-byte-row box per operand) and roles are those of the head's
 // kernels (lmce_engine.cuh, lmce_bwd_pair.cuh).
 //
-// With training the epilogue also keeps g and u in fp32, in blocks of 32 tokens x 32 features
-// laid out as the accumulator is read ([g | u][8 column groups of 4][32 tokens][4]), so each
-// store instruction of a warp writes 512 contiguous bytes. fp32 because dg and du are rounded
-// once already: a gradient's error is sqrt(2) times that of its own rounding alone, and would be
-// 1.8 times with g and u in the inputs' type. The bytes are those an eager block keeps for its
-// backward (g, u, act(g) and h at 2 bytes each). The stores cost the forward 10% (8192 x 4096 x
-// 14336) to 45% (4096 x 896 x 4864), in proportion to their bytes and alike when all of them hit
-// L2: they share the SM's path with the operands.
+// With training the epilogue also keeps g and u, the upper 24 bits of their fp32 values, in
+// blocks of 32 tokens x 32 features laid out as the accumulator is read: for each of g and u the
+// upper 16 bits [4 groups of 8 features][32 tokens][8] and the next 8 bits [2 groups of 16][32
+// tokens][16], so each store instruction of a warp writes 512 contiguous bytes. That leaves an
+// error of at most 2^-15, an eighth of fp16's. dg and du are rounded once already, so a gradient's error is
+// sqrt(2) times that of its own rounding alone; with g and u in the inputs' type it would be 1.8
+// times. 6 bytes per token and feature; an eager block keeps 8 (g, u, act(g) and h). The stores
+// cost the forward their bytes at about 5.5 TB/s whatever their order, and alike when all of
+// them hit L2: they share the SM's path with the operands (with 32 bits kept, 8192 x 4096 x 14336
+// took 10% longer than without, 4096 x 896 x 4864 45%).
 //
 // e4m3 operands (serving): the same kernel with kind::f8f6f4, K = 256 per stage in the same
 // bytes; g and u are scaled by the row's and the feature's scale in the epilogue.
@@ -38,7 +40,10 @@
 namespace lmce {
 
 constexpr int GT_GROUP = 8;        // row blocks that share a sweep over the column blocks
-constexpr int GATED_SAVE_BLOCK = 32 * 32;
+// One 32 x 32 block of saved g and u: 2 KB of upper halves and 1 KB of third bytes for each.
+constexpr int GATED_SAVE_HI = 32 * 32 * 2;
+constexpr int GATED_SAVE_PART = 32 * 32 * 3;
+constexpr int GATED_SAVE_BLOCK = 2 * GATED_SAVE_PART;
 
 enum : int { ACT_SILU = 0, ACT_GELU_TANH = 1 };
 
@@ -46,7 +51,7 @@ struct GatedParams {
   int N, H, F;
   int act;
   int b_rows;            // up to 128 tokens: token rows per stage, N rounded up to 16
-  float* saved;          // SAVE: blocks of 2 x 1024 fp32
+  uint8_t* saved;        // SAVE: blocks of GATED_SAVE_BLOCK bytes
   const float* x_scale;  // e4m3: [N]
   const float* g_scale;  // e4m3: [F]
   const float* u_scale;
@@ -56,27 +61,60 @@ struct GatedParams {
 
 // ------------------------------------------------------------- activation ---
 
-// sig = 1 / (1 + e), e = exp(-v), and v.
-__device__ __forceinline__ float act_sigmoid(float g, int act, float& e) {
+// sig(v) = 1 / (1 + exp(-v)); exp overflows to infinity and sig to 0 far out.
+__device__ __forceinline__ float act_sigmoid(float g, int act) {
   const float v = act == ACT_SILU ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
-  e = ex2_approx(-v * LOG2E);
-  return __fdividef(1.0f, 1.0f + e);
+  return rcp_approx(1.0f + ex2_approx(-LOG2E * v));
 }
 
-__device__ __forceinline__ float act_value(float g, int act) {
-  float e;
-  return g * act_sigmoid(g, act, e);
-}
+__device__ __forceinline__ float act_value(float g, int act) { return g * act_sigmoid(g, act); }
 
-// act(g) and act'(g) = sig + g sig (1 - sig) v'
+// act(g) and act'(g) = sig + g sig (1 - sig) v'. With a = g sig, a - a sig in one rounding keeps
+// the small a (1 - sig) of large g, and is 0 once sig is 1.
 __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
-  float e;
-  const float s = act_sigmoid(g, act, e);
-  const float om = e < 1e30f ? e * s : 1.0f;  // 1 - sig, without its cancellation
-  const float dv = act == ACT_SILU ? 1.0f : 1.5957691216057308f * fmaf(0.134145f * g, g, 1.0f);
+  const float s = act_sigmoid(g, act);
   a = g * s;
-  const float t = a * om;
-  da = t == 0.f ? s : fmaf(t, dv, s);  // far out sig or 1 - sig is 0 and v' may be infinite
+  const float t = fmaf(-a, s, a);
+  if (act == ACT_SILU) {
+    da = t + s;
+  } else {
+    const float dv = 1.5957691216057308f * fmaf(0.134145f * g, g, 1.0f);
+    da = t == 0.f ? s : fmaf(t, dv, s);  // far out v' may be infinite
+  }
+}
+
+// One token's 32 values of a saved block (`dst`: the token's first 16 bytes).
+__device__ __forceinline__ void save_part(uint8_t* dst, const uint32_t (&v)[32]) {
+  uint4* hi = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    hi[i * 32] = make_uint4(
+        __byte_perm(v[8 * i], v[8 * i + 1], 0x7632), __byte_perm(v[8 * i + 2], v[8 * i + 3], 0x7632),
+        __byte_perm(v[8 * i + 4], v[8 * i + 5], 0x7632), __byte_perm(v[8 * i + 6], v[8 * i + 7], 0x7632));
+  uint4* lo = reinterpret_cast<uint4*>(dst + GATED_SAVE_HI);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = 16 * i + 4 * k;
+      w[k] = __byte_perm(__byte_perm(v[j], v[j + 1], 0x0051), __byte_perm(v[j + 2], v[j + 3], 0x0051), 0x5410);
+    }
+    lo[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// The 16 values that two 16-byte pieces of upper halves and one of third bytes hold. The third
+// byte stands in for the lost fourth as well: as good as random, it leaves the values without a
+// bias (an error of at most 2^-15, 0.41 * 2^-15 rms), and zeros, infinities and NaNs as they were.
+__device__ __forceinline__ void load_part(const uint4 (&hi)[2], const uint4& lo, float* f) {
+  const uint32_t h[8] = {hi[0].x, hi[0].y, hi[0].z, hi[0].w, hi[1].x, hi[1].y, hi[1].z, hi[1].w};
+  const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint32_t sel = ((j & 1) ? 0x3200u : 0x1000u) | ((4u + (j & 3)) * 0x11u);
+    f[j] = __uint_as_float(__byte_perm(h[j >> 1], l[j >> 2], sel));
+  }
 }
 
 // ------------------------------------------------------------ few tokens ---
@@ -387,13 +425,9 @@ __global__ void __launch_bounds__(P_THREADS, 1)
           }
         }
         if constexpr (SAVE) {
-          uint4* sv = reinterpret_cast<uint4*>(p.saved) +
-                      (static_cast<size_t>(row0 / 32) * fblocks + f0 / 32) * (2 * GATED_SAVE_BLOCK / 4) + lane;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sv[j * 32] = make_uint4(rg[4 * j], rg[4 * j + 1], rg[4 * j + 2], rg[4 * j + 3]);
-            sv[256 + j * 32] = make_uint4(ru[4 * j], ru[4 * j + 1], ru[4 * j + 2], ru[4 * j + 3]);
-          }
+          uint8_t* blk = p.saved + (static_cast<size_t>(row0 / 32) * fblocks + f0 / 32) * GATED_SAVE_BLOCK + lane * 16;
+          save_part(blk, rg);
+          save_part(blk + GATED_SAVE_PART, ru);
         }
         float v[32];
 #pragma unroll
@@ -654,10 +688,15 @@ __global__ void __launch_bounds__(P_THREADS, 1)
               u *= xs;
             }
             if constexpr (SAVE) {
-              float* sv = p.saved + (static_cast<size_t>(t / 32) * (p.F / 32) + f / 32) * (2 * GATED_SAVE_BLOCK) +
-                          (f % 32) / 4 * 128 + (t % 32) * 4 + f % 4;
-              sv[0] = g;
-              sv[GATED_SAVE_BLOCK] = u;
+              uint8_t* blk = p.saved + (static_cast<size_t>(t / 32) * (p.F / 32) + f / 32) * GATED_SAVE_BLOCK;
+              const int fl = f % 32, tl = t % 32;
+              const int hi = fl / 8 * 512 + tl * 16 + fl % 8 * 2;
+              const int lo = GATED_SAVE_HI + fl / 16 * 512 + tl * 16 + fl % 16;
+              const uint32_t gb = __float_as_uint(g), ub = __float_as_uint(u);
+              *reinterpret_cast<uint16_t*>(blk + hi) = static_cast<uint16_t>(gb >> 16);
+              *reinterpret_cast<uint16_t*>(blk + GATED_SAVE_PART + hi) = static_cast<uint16_t>(ub >> 16);
+              blk[lo] = static_cast<uint8_t>(gb >> 8);
+              blk[GATED_SAVE_PART + lo] = static_cast<uint8_t>(ub >> 8);
             }
             h[static_cast<size_t>(t) * p.F + f] =
                 static_cast<uint16_t>(pack2<BF16>(act_value(g, p.act) * u, 0.f) & 0xffffu);
@@ -692,49 +731,59 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 // A block of four warps per 32 tokens x 64 features (two of the saved blocks), 16 features per
 // warp and one token per lane: g and u arrive as they were stored (512 contiguous bytes per
 // load); dh and the results pass through shared memory, 128 contiguous bytes per token in global
-// memory and a 144-byte pitch here (conflict-free by row and by column). Memory-bound, 14 bytes
-// per element. 16 features keep a thread within 64 registers, so that 32 warps per SM cover each
-// other's loads.
+// memory and a 144-byte pitch here (conflict-free by row and by column). Memory-bound, 12 bytes
+// per element. The next tile's loads are in flight while one is computed and written.
 constexpr int GATED_DACT_THREADS = 128;
-template <bool BF16>
-__global__ void __launch_bounds__(GATED_DACT_THREADS, 8)
-    gated_dact_kernel(const float4* __restrict__ saved, const uint4* __restrict__ dh, int n, int f, int act,
+template <bool BF16, int ACT>
+__global__ void __launch_bounds__(GATED_DACT_THREADS, 5)
+    gated_dact_kernel(const uint8_t* __restrict__ saved, const uint4* __restrict__ dh, int n, int f,
                       uint4* __restrict__ dg, uint4* __restrict__ du) {
   __shared__ uint4 st[2][32][9];  // dh, then dg; du
+  constexpr int PART = GATED_SAVE_PART / 16;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int tf = f / 64, vec = f / 8;
   const long long tiles = static_cast<long long>((n + 31) / 32) * tf;
   const int r0 = threadIdx.x >> 3, c = threadIdx.x & 7;  // global accesses: rows r0 and r0 + 16
-  for (long long b = blockIdx.x; b < tiles; b += gridDim.x) {
+  uint4 gh[2], uh[2], gl, ul, d0, d1;
+  const auto load = [&](long long b) {
     const int rb = static_cast<int>(b / tf), cb = static_cast<int>(b - static_cast<long long>(rb) * tf);
-    const long long blk = static_cast<long long>(rb) * (f / 32) + cb * 2 + (warp >> 1);
-    const float4* sv = saved + blk * (2 * GATED_SAVE_BLOCK / 4) + (warp & 1) * 128 + lane;
+    const uint8_t* blk = saved + (static_cast<long long>(rb) * (f / 32) + cb * 2 + (warp >> 1)) * GATED_SAVE_BLOCK;
+    const uint4* hi = reinterpret_cast<const uint4*>(blk) + (warp & 1) * 64 + lane;
+    const uint4* lo = reinterpret_cast<const uint4*>(blk + GATED_SAVE_HI) + (warp & 1) * 32 + lane;
+    const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 8 + c;
+    d0 = d1 = make_uint4(0u, 0u, 0u, 0u);
+    if (rb * 32 + r0 < n) d0 = __ldcs(dh + at);
+    if (rb * 32 + r0 + 16 < n) d1 = __ldcs(dh + at + 16ll * vec);
+    gh[0] = __ldcs(hi);
+    gh[1] = __ldcs(hi + 32);
+    gl = __ldcs(lo);
+    uh[0] = __ldcs(hi + PART);
+    uh[1] = __ldcs(hi + PART + 32);
+    ul = __ldcs(lo + PART);
+  };
+  long long b = blockIdx.x;
+  if (b < tiles) load(b);
+  for (; b < tiles; b += gridDim.x) {
+    const int rb = static_cast<int>(b / tf), cb = static_cast<int>(b - static_cast<long long>(rb) * tf);
     const long long at = (static_cast<long long>(rb) * 32 + r0) * vec + cb * 8 + c;
     const bool live0 = rb * 32 + r0 < n, live1 = rb * 32 + r0 + 16 < n;
-    float4 g[4], u[4];
-    uint4 d0 = make_uint4(0u, 0u, 0u, 0u), d1 = d0;
-    if (live0) d0 = __ldcs(dh + at);
-    if (live1) d1 = __ldcs(dh + at + 16ll * vec);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = __ldcs(sv + j * 32);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = __ldcs(sv + 256 + j * 32);
     st[0][r0][c] = d0;
     st[0][r0 + 16][c] = d1;
     __syncthreads();
-    float d[16], e[16];
+    float d[16], e[16], g[16], u[16];
     uint4* own0 = &st[0][lane][warp * 2];
     uint4* own1 = &st[1][lane][warp * 2];
     unpack8<BF16>(own0[0], d);
     unpack8<BF16>(own0[1], d + 8);
-    const float* gf = reinterpret_cast<const float*>(g);
-    const float* uf = reinterpret_cast<const float*>(u);
+    load_part(gh, gl, g);
+    load_part(uh, ul, u);
+    if (b + gridDim.x < tiles) load(b + gridDim.x);  // in flight while this tile is computed and written
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       float a, da;
-      act_both(gf[j], act, a, da);
+      act_both(g[j], ACT, a, da);
       e[j] = d[j] * a;
-      d[j] = d[j] * uf[j] * da;
+      d[j] = d[j] * u[j] * da;
     }
     own0[0] = pack8<BF16>(d);
     own0[1] = pack8<BF16>(d + 8);

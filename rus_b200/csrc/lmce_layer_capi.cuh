@@ -415,7 +415,7 @@ int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t
 
 size_t lmce_gated_saved_bytes(int64_t n_rows, int64_t ffn_dim) {
   if (n_rows <= 0 || ffn_dim <= 0) return 0;
-  return static_cast<size_t>((n_rows + 31) / 32 * 32) * ffn_dim * 8;
+  return static_cast<size_t>((n_rows + 31) / 32 * 32) * ffn_dim * 6;
 }
 
 int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64_t n_rows, int64_t hidden_dim,
@@ -434,7 +434,7 @@ int lmce_gated_linear(const void* x, const void* w_gate, const void* w_up, int64
   p.H = static_cast<int>(hidden_dim);
   p.F = static_cast<int>(ffn_dim);
   p.act = act;
-  p.saved = static_cast<float*>(saved);
+  p.saved = static_cast<uint8_t*>(saved);
   p.err = d->err_ptr;
   p.timeout_ns = wait_timeout_ns();
   if (n_rows == 1 && !saved)
@@ -519,15 +519,13 @@ int lmce_gated_backward(const void* d_h, const void* saved, const void* x, const
   const int64_t n = n_rows, h = hidden_dim, f = ffn_dim;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
-  const int dgrid = static_cast<int>(std::min<int64_t>((n + 31) / 32 * (f / 64), d->sms * 8ll));
-  if (bf16)
-    gated_dact_kernel<true><<<dgrid, GATED_DACT_THREADS, 0, st>>>(
-        static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
-        act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
-  else
-    gated_dact_kernel<false><<<dgrid, GATED_DACT_THREADS, 0, st>>>(
-        static_cast<const float4*>(saved), static_cast<const uint4*>(d_h), static_cast<int>(n), static_cast<int>(f),
-        act, static_cast<uint4*>(dg), static_cast<uint4*>(du));
+  const int dgrid = static_cast<int>(std::min<int64_t>((n + 31) / 32 * (f / 64), d->sms * 5ll));
+  const bool silu = act == LMCE_ACT_SILU;
+  const auto dact = bf16 ? (silu ? gated_dact_kernel<true, ACT_SILU> : gated_dact_kernel<true, ACT_GELU_TANH>)
+                         : (silu ? gated_dact_kernel<false, ACT_SILU> : gated_dact_kernel<false, ACT_GELU_TANH>);
+  dact<<<dgrid, GATED_DACT_THREADS, 0, st>>>(static_cast<const uint8_t*>(saved), static_cast<const uint4*>(d_h),
+                                             static_cast<int>(n), static_cast<int>(f), static_cast<uint4*>(dg),
+                                             static_cast<uint4*>(du));
   if (int rc = launched()) return rc;
 
   CUtensorMap maps[8];

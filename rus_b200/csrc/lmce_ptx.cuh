@@ -33,6 +33,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// 1 / x on the SFU (MUFU.RCP); 0 for infinities and for x beyond 2^126.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // log2(x) on the SFU.
 __device__ __forceinline__ float lg2_approx(float x) {
   float y;

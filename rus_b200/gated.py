@@ -91,8 +91,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     64, any number of tokens. ``activation``: ``"silu"`` or ``"gelu_tanh"``. Products
     accumulate and the activation runs in fp32; the result is rounded once. Differentiable in
     ``x`` and both weights (each gradient is computed only if its tensor wants it). When a
-    gradient is wanted the forward keeps both products in fp32, 8 bytes per token and
-    feature, for the backward; ``torch.utils.checkpoint`` around the block trades that for a
+    gradient is wanted the forward keeps both products, 24 bits of each, 6 bytes per token
+    and feature, for the backward; ``torch.utils.checkpoint`` around the block trades that for a
     second forward."""
     _check(x, w_gate, w_up, activation, "gated_linear", 64)
     if x.dtype not in _DTYPES:

@@ -95,6 +95,8 @@ def test_gradients(cuda_device, n, h, f, dtype, kind):
     # |act''| <= 0.8 and |act'| <= 1.13, and 2^-18 for the terms sig and g sig (1 - sig) v', each
     # at most 1.2, of act'. Where act' is near its zero (g = -1.28 for silu, -0.75 for gelu) the last
     # three are larger than eps / 2 of the small value.
+    # That 24 bits of g and u are kept adds 2^-15 of them at most, an eighth of fp16's eps / 2: it has
+    # no term of its own, the six norms below are taken without it.
     eg = xd.norm(dim=1)[:, None] * gd.norm(dim=1) * 2 ** -18
     eu = xd.norm(dim=1)[:, None] * ud.norm(dim=1) * 2 ** -18
     floor = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps

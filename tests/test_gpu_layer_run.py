@@ -209,7 +209,7 @@ def test_offsets_beyond_32_bits(cuda_device):
     assert (p.grad[tail] == want.item()).all() and (p.grad[:700] == want.item()).all()
     del p, x
     torch.cuda.empty_cache()
-    n, h, f = 150_100, 64, 14400  # h and both of dg and du over 2^31 elements, 17 GB of saved products
+    n, h, f = 150_100, 64, 14400  # h and both of dg and du over 2^31 elements, 13 GB of kept products
     x = torch.randn(n, h, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
     wg, wu = (torch.randn(f, h, device=cuda_device, dtype=torch.bfloat16) * h ** -0.5 for _ in range(2))
     out = gated_linear(x, wg, wu)

@@ -106,7 +106,7 @@ def test_clip_entry():
 
 def test_workspaces():
     lib = _lib.load()
-    assert lib.lmce_gated_saved_bytes(33, 64) == 64 * 64 * 8  # tokens in blocks of 32
+    assert lib.lmce_gated_saved_bytes(33, 64) == 64 * 64 * 6  # tokens in blocks of 32
     assert lib.lmce_gated_saved_bytes(0, 64) == 0 and lib.lmce_clip_grad_workspace_bytes(0) == 0
     assert lib.lmce_add_rmsnorm_bwd_workspace_bytes(5, 64) == 5 * 64 * 4
     # the partial rows of the norm's weight gradient do not grow with the tokens
