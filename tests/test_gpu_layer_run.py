@@ -138,6 +138,49 @@ def test_serving_chain_on_e4m3(cuda_device, n):
     assert (h.double() - full).norm() <= full.norm() * 2 ** -4
 
 
+def _all_operators(dev, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    x, r = (torch.randn(400, 256, device=dev, generator=g).bfloat16().requires_grad_(True) for _ in range(2))
+    w = torch.ones(256, device=dev).bfloat16().requires_grad_(True)
+    wg, wu = ((torch.randn(320, 256, device=dev, generator=g) / 16).bfloat16().requires_grad_(True) for _ in range(2))
+    y, s = add_rms_norm(x, r, w)
+    h = gated_linear(y, wg, wu)
+    (h.float().square().sum() + s.float().sum()).backward()
+    total = clip_grad_norm_([x, r, w, wg, wu], 1.0)
+    with torch.no_grad():
+        q, scale, _ = add_rms_norm_e4m3(x, r, w)
+    return [t.detach().float() for t in (y, s, h, x.grad, r.grad, w.grad, wg.grad, wu.grad, total, q, scale)]
+
+
+def test_threads_on_streams_of_their_own(cuda_device):
+    from concurrent.futures import ThreadPoolExecutor
+
+    want = [_all_operators(cuda_device, i) for i in range(4)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            out = [_all_operators(cuda_device, i) for _ in range(3)]
+        stream.synchronize()
+        return out
+
+    with ThreadPoolExecutor(4) as pool:
+        for i, runs in enumerate(pool.map(work, range(4))):
+            for got in runs:
+                assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+    assert _lib.device_error() == 0
+
+
+def test_another_device_is_current(cuda_device, monkeypatch):
+    """With one GPU: the path that makes the tensors' device current, taken by a current device
+    that claims to be another."""
+    want = _all_operators(cuda_device, 9)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: cuda_device.index + 1)
+    got = _all_operators(cuda_device, 9)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals_on_the_device(cuda_device):
     dev = cuda_device
     x, w = torch.randn(4, 128, device=dev).half(), torch.ones(128, device=dev).half()
