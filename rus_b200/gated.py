@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .norm import _rows, no_second_order
-from .ops import _DTYPES, _ptr
+from .ops import _DTYPES, _debug_sync, _ptr, _raise_device_error
 
 ACTIVATIONS = {"silu": _lib.LMCE_ACT_SILU, "gelu_tanh": _lib.LMCE_ACT_GELU_TANH}
 
@@ -51,6 +51,8 @@ def _forward(x, w_gate, w_up, activation, save: bool):
             saved = xc.new_empty(int(_lib.load().lmce_gated_saved_bytes(n, f)), dtype=torch.uint8)
         _lib.launch(x.device, "lmce_gated_linear", xc.data_ptr(), wg.data_ptr(), wu.data_ptr(), n, h, f,
                     _DTYPES[x.dtype], ACTIVATIONS[activation], out.data_ptr(), _ptr(saved))
+        if _debug_sync():
+            _raise_device_error()
     return out, xc, wg, wu, saved
 
 
@@ -81,6 +83,8 @@ class GatedLinearFn(torch.autograd.Function):
             _lib.launch(dev, "lmce_gated_backward", g.data_ptr(), saved.data_ptr(), x.data_ptr(), wg.data_ptr(),
                         wu.data_ptr(), n, h, f, _DTYPES[x.dtype], ACTIVATIONS[ctx.activation], _ptr(dx), _ptr(dg),
                         _ptr(du), ws.data_ptr(), ws_bytes)
+            if _debug_sync():
+                _raise_device_error()
         return dx, dg, du, None
 
 
@@ -138,4 +142,6 @@ def gated_linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w_gate: torch.Tens
         _lib.launch(x.device, "lmce_gated_linear_e4m3", xc.data_ptr(), sx.data_ptr(), wg.data_ptr(), sg.data_ptr(),
                     wu.data_ptr(), su.data_ptr(), n, h, f, _DTYPES[out_dtype], ACTIVATIONS[activation],
                     out.data_ptr())
+        if _debug_sync():
+            _raise_device_error()
     return out
