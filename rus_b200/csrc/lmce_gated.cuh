@@ -488,6 +488,8 @@ __global__ void __launch_bounds__(P_THREADS, 1)
 // A stage is K = 128 (256 for e4m3): per 128-byte column block the gate rows and the up rows
 // follow one another, four 8 KB boxes. Lanes 0-63 of the accumulator are gate features, 64-127
 // the same features of up: the up warps hand their values over through shared memory.
+// Against the pairs at the border (bf16): 128 tokens here 15.4 us at 1536 x 8960 and 50.4 us at
+// 4096 x 14336, 129 tokens there 16.4 and 64.4 us.
 constexpr int GF_FT = 64;
 constexpr int GF_W_BYTES = 2 * GF_FT * 2 * 128;          // 32 KB of weights per stage
 constexpr int GF_MAX_STAGES = 5;

@@ -23,12 +23,14 @@ struct RowShape {
   int vpt, threads, rows;
 };
 
-// Threads and vectors per thread for a row of `vec` 16-byte vectors: one vector per thread
-// while rows are few (latency), two when there are enough rows to fill the SMs (more loads in
-// flight per thread), four where a row would need over 512 threads.
+// Threads and vectors per thread for a row of `vec` 16-byte vectors: one vector per thread while
+// that is under 700 threads per SM (latency), two beyond (more loads in flight per thread), four
+// where a row would need over 512 threads. One B200, forward, one and two vectors: 1 x 896 1.77
+// and 2.02 us, 512 x 896 3.04 and 3.36, 300 x 4096 4.56 and 4.40 (e4m3 5.55 and 4.31), 32768 x
+// 4096 200 and 169 (four: 178).
 RowShape row_shape(int64_t n, int vec, int sms) {
   RowShape s;
-  s.vpt = n > 4ll * sms && vec > 32 ? 2 : 1;
+  s.vpt = n * vec > 700ll * sms && vec > 32 ? 2 : 1;
   const auto threads = [&] { return (vec + 32 * s.vpt - 1) / (32 * s.vpt) * 32; };
   while (threads() > kAnThreads) s.vpt *= 2;
   s.threads = threads();
