@@ -20,13 +20,13 @@
 // With training the epilogue also keeps g and u, the upper 24 bits of their fp32 values, in
 // blocks of 32 tokens x 32 features laid out as the accumulator is read: for each of g and u the
 // upper 16 bits [4 groups of 8 features][32 tokens][8] and the next 8 bits [2 groups of 16][32
-// tokens][16], so each store instruction of a warp writes 512 contiguous bytes. That leaves an
-// error of at most 2^-15, an eighth of fp16's. dg and du are rounded once already, so a gradient's error is
-// sqrt(2) times that of its own rounding alone; with g and u in the inputs' type it would be 1.8
-// times. 6 bytes per token and feature; an eager block keeps 8 (g, u, act(g) and h). The stores
-// cost the forward their bytes at about 5.5 TB/s whatever their order, and alike when all of
-// them hit L2: they share the SM's path with the operands (with 32 bits kept, 8192 x 4096 x 14336
-// took 10% longer than without, 4096 x 896 x 4864 45%).
+// tokens][16], one contiguous piece of 3 KB each. That leaves an error of at most 2^-15, an eighth
+// of fp16's. dg and du are rounded once already, so a gradient's error is sqrt(2) times that of its
+// own rounding alone; with g and u in the inputs' type it would be 1.8 times. 6 bytes per token and
+// feature; an eager block keeps 8 (g, u, act(g) and h). The pieces leave by bulk stores from
+// shared memory: with 16-byte stores from registers the warps waited on the SM's path to L2 (one
+// B200, 8192 x 4096 x 14336 1500 us without, 1633 with register stores, 1556 with bulk stores; 2048
+// x 1536 x 8960 96, 113 and 105; 4096 x 896 x 4864 63, 84 and 81).
 //
 // e4m3 operands (serving): the same kernel with kind::f8f6f4, K = 256 per stage in the same
 // bytes; g and u are scaled by the row's and the feature's scale in the epilogue.
@@ -42,7 +42,8 @@ namespace lmce {
 constexpr int GT_GROUP = 8;        // row blocks that share a sweep over the column blocks
 // One 32 x 32 block of saved g and u: 2 KB of upper halves and 1 KB of third bytes for each.
 constexpr int GATED_SAVE_HI = 32 * 32 * 2;
-constexpr int GATED_SAVE_PART = 32 * 32 * 3;
+constexpr int GATED_SAVE_LO = 32 * 32;
+constexpr int GATED_SAVE_PART = GATED_SAVE_HI + GATED_SAVE_LO;
 constexpr int GATED_SAVE_BLOCK = 2 * GATED_SAVE_PART;
 
 enum : int { ACT_SILU = 0, ACT_GELU_TANH = 1 };
@@ -83,7 +84,7 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) 
   }
 }
 
-// One token's 32 values of a saved block (`dst`: the token's first 16 bytes).
+// One token's 32 values in a saved block's layout (`dst`: the token's first 16 bytes).
 __device__ __forceinline__ void save_part(uint8_t* dst, const uint32_t (&v)[32]) {
   uint4* hi = reinterpret_cast<uint4*>(dst);
 #pragma unroll
@@ -424,29 +425,55 @@ __global__ void __launch_bounds__(P_THREADS, 1)
             }
           }
         }
-        if constexpr (SAVE) {
-          uint8_t* blk = p.saved + (static_cast<size_t>(row0 / 32) * fblocks + f0 / 32) * GATED_SAVE_BLOCK + lane * 16;
-          save_part(blk, rg);
-          save_part(blk + GATED_SAVE_PART, ru);
-        }
+        // What leaves goes through two 2 KB halves of the warp's slice in turn, each written once the
+        // store of two before has read it.
+        const auto next_half = [&]() {
+          uint8_t* box = xstage + half * 2048;
+          half ^= 1;
+          if (lane == 0) bulk_wait_read_1();
+          __syncwarp();
+          return box;
+        };
+        const auto written = [&]() {
+          fence_async_shared();
+          __syncwarp();
+          return lane == 0;
+        };
         float v[32];
+        if constexpr (SAVE) {
+          // g's 3 KB, then u's, through the slice (two 2 KB halves in turn, which waits less at each
+          // step, is as fast for few stages and 1-4% slower for many)
+          uint8_t* blk = p.saved + (static_cast<size_t>(row0 / 32) * fblocks + f0 / 32) * GATED_SAVE_BLOCK;
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          save_part(xstage + lane * 16, rg);
+          if (written()) {
+            bulk_store(blk, xstage, GATED_SAVE_PART);
+            bulk_commit_group();
+          }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = act_value(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
-        // one TMA store of the warp's 32 tokens x 32 features, through two 2 KB halves of its
-        // slice in turn (64-byte swizzle); tokens past N are clipped
-        uint8_t* box = xstage + half * 2048;
-        half ^= 1;
-        if (lane == 0) bulk_wait_read_1();
-        __syncwarp();
+          for (int j = 0; j < 32; ++j) v[j] = act_value(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          save_part(xstage + lane * 16, ru);
+          if (written()) {
+            bulk_store(blk + GATED_SAVE_PART, xstage, GATED_SAVE_PART);
+            bulk_commit_group();
+            bulk_wait_read_all();
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = act_value(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
+        }
+        // the warp's 32 tokens x 32 features of h, a 64-byte-swizzled box; tokens past N are clipped
+        uint8_t* box = next_half();
         uint4* row = reinterpret_cast<uint4*>(box + lane * 64);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           row[i ^ ((lane >> 1) & 3)] =
               make_uint4(pack2<BF16>(v[8 * i], v[8 * i + 1]), pack2<BF16>(v[8 * i + 2], v[8 * i + 3]),
                          pack2<BF16>(v[8 * i + 4], v[8 * i + 5]), pack2<BF16>(v[8 * i + 6], v[8 * i + 7]));
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
+        if (written()) {
           tma_store_2d(&map_h, box, f0, row0);
           bulk_commit_group();
         }

@@ -159,6 +159,14 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                : "memory");
 }
 
+// Plain (untiled) bulk copy of `bytes` contiguous bytes of this CTA's shared memory to global
+// memory, tracked by the thread's bulk async-group; addresses and size multiples of 16.
+__device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(smem_src)),
+               "r"(bytes)
+               : "memory");
+}
+
 // 2-D tiled bulk-tensor store shared -> global (this GPU's memory), tracked by the
 // thread's bulk async-group. x (innermost, elements) times the element size must be a
 // multiple of 16 bytes; both coordinates must be non-negative.
