@@ -7,6 +7,7 @@ raises. Status codes are mapped to ``LmceError`` with the library's message.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import threading
 from pathlib import Path
 
@@ -166,19 +167,27 @@ def call(name: str, *args) -> int:
     return rc
 
 
-def launch(device, name: str, *args) -> None:
-    """Call ``name`` (whose last argument is the stream) on ``device``'s current stream, with
-    ``device`` current. The short way of small operators, whose time is the host's: no context
-    manager where the device is current already, and the stream's handle without its object."""
-    fn = getattr(_lib or load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
-    if rc != LMCE_OK:
-        check(rc)
+_host = None
+
+
+def host():
+    """The C++ host side of the operators around the head (``_host.so``), bound to the library."""
+    global _host
+    lib = load()
+    with _lock:
+        if _host is None:
+            try:
+                mod = importlib.import_module("._host", __package__)
+            except ImportError as e:
+                raise LmceError(LMCE_ERR_UNSUPPORTED,
+                                f"_host.so cannot be loaded: build it with `python -m rus_b200.build` ({e})") from e
+            if mod.torch_version != torch.__version__.split("+")[0]:
+                raise LmceError(LMCE_ERR_UNSUPPORTED,
+                                f"_host.so was built for torch {mod.torch_version}, not {torch.__version__}: "
+                                "rebuild it with `python -m rus_b200.build`")
+            mod.init(lib._name, LmceError)
+            _host = mod
+        return _host
 
 
 def launch_count() -> int:

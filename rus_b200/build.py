@@ -1,4 +1,6 @@
-"""Builds the in-tree C-ABI library ``rus_b200/liblmce.so`` with nvcc for sm_100a.
+"""Builds the in-tree C-ABI library ``rus_b200/liblmce.so`` with nvcc for sm_100a, and
+``rus_b200/_host.so``, the C++ host side of the operators around the head, with g++
+against torch's headers.
 
 The library is compiled ahead of time (no JIT cache), so the built ``.so``
 travels with the source tree. ``python -m rus_b200.build`` rebuilds it.
@@ -9,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -17,6 +20,8 @@ INCLUDE = PKG_DIR.parent / "include"
 LIB_PATH = PKG_DIR / "liblmce.so"
 SOURCES = [CSRC / "lmce_capi.cu"]
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "lmce.h"]
+HOST_PATH = PKG_DIR / "_host.so"
+HOST_DEPS = [CSRC / "lmce_host.cpp", INCLUDE / "lmce.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -49,24 +54,54 @@ def compile_command(out: Path = LIB_PATH, extra: list[str] | None = None) -> lis
     ]
 
 
-def needs_build(out: Path = LIB_PATH) -> bool:
+def host_command(out: Path = HOST_PATH) -> list[str]:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    includes = [INCLUDE, root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                sysconfig.get_paths()["include"]]
+    return [
+        os.environ.get("CXX") or "g++",
+        "-O2",
+        "-std=c++17",
+        "-shared",
+        "-fPIC",
+        "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[f"-I{p}" for p in includes],
+        str(CSRC / "lmce_host.cpp"),
+        "-o",
+        str(out),
+        f"-L{root / 'lib'}",
+        "-ltorch",
+        "-ltorch_cpu",
+        "-lc10",
+        "-lc10_cuda",
+        "-ltorch_python",
+        "-ldl",
+    ]
+
+
+def needs_build(out: Path = LIB_PATH, deps: list[Path] = DEPS) -> bool:
     if not out.exists():
         return True
     mtime = out.stat().st_mtime
-    return any(dep.stat().st_mtime > mtime for dep in DEPS)
+    return any(dep.stat().st_mtime > mtime for dep in deps)
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """Compile liblmce.so if it is missing or older than its sources."""
-    if not force and not needs_build():
-        return LIB_PATH
-    cmd = compile_command()
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd[cmd.index("-o") + 1] = str(tmp)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB_PATH)
+    """Compile liblmce.so and _host.so where they are missing or older than their sources."""
+    for out, deps, command in ((LIB_PATH, DEPS, compile_command), (HOST_PATH, HOST_DEPS, host_command)):
+        if not force and not needs_build(out, deps):
+            continue
+        cmd = command()
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        tmp = out.with_suffix(".so.tmp")
+        cmd[cmd.index("-o") + 1] = str(tmp)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, out)
     return LIB_PATH
 
 

@@ -206,8 +206,9 @@ int launch_gated_token(const void* x, const void* wg, const void* wu, const Gate
 int check_gated(int64_t n, int64_t h, int64_t f, int dtype, int act, int64_t h_step) {
   if (n <= 0 || n > kGatedMaxRows) return fail(LMCE_ERR_INVALID_ARGUMENT, "bad n_rows");
   if (h <= 0 || h % h_step != 0 || h > kGatedMaxDim)
-    return fail(LMCE_ERR_UNSUPPORTED, "hidden_dim must be a multiple of %lld", (long long)h_step);
-  if (f <= 0 || f % 64 != 0 || f > kGatedMaxDim) return fail(LMCE_ERR_UNSUPPORTED, "ffn_dim must be a multiple of 64");
+    return fail(LMCE_ERR_UNSUPPORTED, "hidden_dim must be a multiple of %lld, at most 2^20", (long long)h_step);
+  if (f <= 0 || f % 64 != 0 || f > kGatedMaxDim)
+    return fail(LMCE_ERR_UNSUPPORTED, "ffn_dim must be a multiple of 64, at most 2^20");
   if (((n + 127) / 128) * ((f + 63) / 64) > 0x7fffffffll || ((n + 255) / 256) * ((h + 255) / 256) > 0x3ffffffll)
     return fail(LMCE_ERR_UNSUPPORTED, "too many tiles");
   if (dtype != LMCE_DTYPE_F16 && dtype != LMCE_DTYPE_BF16) return fail(LMCE_ERR_UNSUPPORTED, "dtype %d", dtype);

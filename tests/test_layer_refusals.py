@@ -120,6 +120,24 @@ def test_workspaces():
     assert lib.lmce_gated_bwd_workspace_bytes(1, 1536, 8960, 0, 2) < 1 << 16
 
 
+def test_host_side_loads_and_takes_cuda_tensors_only():
+    host = _lib.host()
+    assert host is _lib.host() and host.torch_version == torch.__version__.split("+")[0]
+    x, w = torch.randn(4, 128).half(), torch.ones(128).half()
+    wg = torch.randn(64, 128).half()
+    q, s4, s64 = x.to(torch.float8_e4m3fn), torch.ones(4), torch.ones(64)
+    assert host.add_rms_norm(x, x, w, 1e-6) is None and host.add_rms_norm_e4m3(x, None, w, 1e-6) is None
+    assert host.gated_linear(x, wg, wg, 0) is None
+    q8 = wg.to(torch.float8_e4m3fn)
+    assert host.gated_linear_e4m3(q, s4, q8, s64, q8, s64, 0, torch.float16) is None
+    p = torch.zeros(4, requires_grad=True)
+    assert host.clip_grad_norm([], 1.0, True) is None and host.clip_grad_norm([p], 1.0, True) is None
+    p.grad = torch.ones(4)
+    assert host.clip_grad_norm([p], 1.0, True) is None and host.clip_grad_norm([p.grad, 3], 1.0, False) is None
+    with pytest.raises(TypeError):
+        host.add_rms_norm(x, x, None, 1e-6)
+
+
 def test_tensors_on_the_cpu():
     x, w = torch.randn(4, 128).half(), torch.ones(128).half()
     wg = torch.randn(64, 128).half()
