@@ -112,6 +112,44 @@ def test_checkpointed_block_gives_the_same_gradients(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(*grads))
 
 
+def test_autograd_modes(cuda_device):
+    """Anomaly detection, offloaded saved tensors, inference mode, a retained graph, memory that is
+    given back, and an output changed in place before the backward."""
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x, r = (torch.randn(300, 256, device=cuda_device, generator=g).half().requires_grad_(True) for _ in range(2))
+    w = torch.ones(256, device=cuda_device).half().requires_grad_(True)
+    wg, wu = ((torch.randn(128, 256, device=cuda_device, generator=g) / 16).half().requires_grad_(True)
+              for _ in range(2))
+    leaves = (x, r, w, wg, wu)
+
+    def loss():
+        y, s = add_rms_norm(x, r, w)
+        return gated_linear(y, wg, wu).float().sum() + s.float().sum()
+
+    want = torch.autograd.grad(loss(), leaves)
+    with torch.autograd.detect_anomaly(check_nan=True):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss(), leaves), want))
+    with torch.autograd.graph.save_on_cpu():
+        value = loss()
+    for retain in (True, False):
+        got = torch.autograd.grad(value, leaves, retain_graph=retain)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        y, s = add_rms_norm(x, r, w)
+        assert y.is_inference() and gated_linear(y, wg, wu).is_inference()
+    del value, got, y, s
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        torch.autograd.grad(loss(), leaves)
+        loss()  # a graph that is dropped without a backward
+    assert torch.cuda.memory_allocated() <= before
+    y, s = add_rms_norm(x, r, w)
+    s.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 @pytest.mark.parametrize("n", [1, 5, 64, 300])
 def test_serving_chain_on_e4m3(cuda_device, n):
     """Residual norm into e4m3, gated projection on e4m3 weights: exactly the product of the
