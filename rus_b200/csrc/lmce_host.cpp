@@ -16,12 +16,15 @@
 #include <torch/version.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <dlfcn.h>
 
 #include <cstdlib>
+#include <functional>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -87,6 +90,15 @@ void no_second_order(const char* who) {
   // autograd runs a backward in grad mode only to differentiate it again
   if (at::GradMode::is_enabled())
     throw std::runtime_error(std::string("LMCE_ERR_UNSUPPORTED: ") + who + ": no second derivative (create_graph=True)");
+}
+
+// None of these operators has a forward-mode derivative, and the plain path would drop a tangent.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
+void no_tangents(const char* who, std::initializer_list<std::reference_wrapper<const Tensor>> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : tensors)
+    if (dual(t)) throw Status(LMCE_ERR_UNSUPPORTED, std::string(who) + ": no forward-mode derivative");
 }
 
 bool is16(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
@@ -187,6 +199,7 @@ bool records(const Tensor& a, const Tensor& b, const std::optional<Tensor>& c) {
 
 std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const std::optional<Tensor>& residual,
                                                        const Tensor& weight, double eps) {
+  no_tangents("add_rms_norm", {x, residual ? *residual : x, weight});
   if (!norm_args(x, residual, weight)) return std::nullopt;
   if (records(x, weight, residual)) {
     variable_list out = NormNode::apply(x, residual, weight, eps);
@@ -199,6 +212,7 @@ std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const st
 std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_e4m3(const Tensor& x,
                                                                     const std::optional<Tensor>& residual,
                                                                     const Tensor& weight, double eps) {
+  no_tangents("add_rms_norm_e4m3", {x, residual ? *residual : x, weight});
   if (!norm_args(x, residual, weight) || records(x, weight, residual)) return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t h = x.size(-1);
@@ -290,6 +304,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
 };
 
 std::optional<Tensor> gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int64_t act) {
+  no_tangents("gated_linear", {x, w_gate, w_up});
   if (!gated_args(x, w_gate, w_up, 64) || !is16(x.scalar_type())) return std::nullopt;
   if (records(x, w_gate, w_up)) return GatedNode::apply(x, w_gate, w_up, act);
   return gated_forward(x, w_gate, w_up, act, false).h;
@@ -298,6 +313,7 @@ std::optional<Tensor> gated_linear(const Tensor& x, const Tensor& w_gate, const 
 std::optional<Tensor> gated_linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& w_gate,
                                         const Tensor& gate_scale, const Tensor& w_up, const Tensor& up_scale,
                                         int64_t act, at::ScalarType out_dtype) {
+  no_tangents("gated_linear_e4m3", {x, x_scale, w_gate, gate_scale, w_up, up_scale});
   if (!gated_args(x, w_gate, w_up, 128) || x.scalar_type() != at::kFloat8_e4m3fn || !is16(out_dtype))
     return std::nullopt;
   const int64_t f = w_gate.size(0), h = w_gate.size(1);
@@ -342,6 +358,7 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
     const Tensor& t0 = THPVariable_Unpack(o);
     const Tensor& g = of_parameters ? t0.grad() : t0;
     if (!g.defined()) continue;
+    no_tangents("clip_grad_norm_", {g});
     const at::ScalarType t = g.scalar_type();
     if (!usable(g) || !(is16(t) || t == at::kFloat) || !g.is_contiguous()) return std::nullopt;
     if (!first.defined())

@@ -1,0 +1,41 @@
+"""GPU: the operators around the head under torch's modes, hooks and unusual calls."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from rus_b200 import (_lib, add_rms_norm, add_rms_norm_e4m3, clip_grad_norm_, gated_linear, gated_linear_e4m3)
+
+pytestmark = pytest.mark.gpu
+
+
+def _e4m3(t):
+    scale = t.float().abs().amax(1) / 448
+    return (t.float() / scale[:, None]).to(torch.float8_e4m3fn), scale
+
+
+def _inputs(dev, n=4, h=128, f=64):
+    g = torch.Generator(device=dev).manual_seed(11)
+    x, r = (torch.randn(n, h, device=dev, generator=g).half() for _ in range(2))
+    w = (1 + 0.1 * torch.randn(h, device=dev, generator=g)).half()
+    wg, wu = ((torch.randn(f, h, device=dev, generator=g) * h ** -0.5).half() for _ in range(2))
+    return x, r, w, wg, wu
+
+
+def test_tangents_are_refused(cuda_device):
+    x, r, w, wg, wu = _inputs(cuda_device)
+    q, sx = _e4m3(x)
+    (g8, sg), (u8, su) = _e4m3(wg), _e4m3(wu)
+    p = torch.zeros(4, device=cuda_device, requires_grad=True)
+    with fwd.dual_level():
+        d = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        p.grad = d(torch.full((4,), 3.0, device=cuda_device))
+        for call in (lambda: add_rms_norm(d(x), r, w), lambda: add_rms_norm(x, d(r), w),
+                     lambda: add_rms_norm(x, None, d(w)), lambda: add_rms_norm_e4m3(d(x), None, w),
+                     lambda: add_rms_norm(d(x), r, w.clone().requires_grad_(True)),
+                     lambda: gated_linear(d(x), wg, wu), lambda: gated_linear(x, wg, d(wu)),
+                     lambda: gated_linear_e4m3(q, d(sx), g8, sg, u8, su), lambda: clip_grad_norm_([p], 1.0)):
+            with pytest.raises(_lib.LmceError, match="forward-mode"):
+                call()
+    assert (p.grad == 3.0).all()
