@@ -8,8 +8,8 @@
 //
 // Every function returns nothing where an argument is not one it takes: the Python module
 // then says what is wrong with it (norm.py, gated.py, clip.py). Errors of the library
-// become the package's LmceError; in a backward, which autograd runs, a RuntimeError with the
-// same text.
+// become the package's LmceError, in a backward as well.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -57,16 +57,9 @@ struct Status : std::runtime_error {
   Status(int code_, const std::string& text) : std::runtime_error(text), code(code_) {}
 };
 
-const char* code_name(int code) {
-  switch (code) {
-    case LMCE_ERR_INVALID_ARGUMENT: return "LMCE_ERR_INVALID_ARGUMENT";
-    case LMCE_ERR_UNSUPPORTED: return "LMCE_ERR_UNSUPPORTED";
-    case LMCE_ERR_CUDA: return "LMCE_ERR_CUDA";
-    case LMCE_ERR_TIMEOUT: return "LMCE_ERR_TIMEOUT";
-    case LMCE_ERR_LABEL_RANGE: return "LMCE_ERR_LABEL_RANGE";
-    case LMCE_ERR_WORKSPACE: return "LMCE_ERR_WORKSPACE";
-  }
-  return "LMCE_ERR";
+py::object& error_type() {
+  static py::object* type = new py::object();  // outlives the interpreter's teardown
+  return *type;
 }
 
 void check(int rc) {
@@ -81,15 +74,20 @@ void check_device() {
   if (rc != LMCE_OK) throw Status(rc, "reported by a kernel");
 }
 
-// In a backward: the error's name goes into the text, since its type is lost on the way.
-void check_backward(int rc) {
-  if (rc != LMCE_OK) throw std::runtime_error(std::string(code_name(rc)) + ": " + lib.lmce_last_error());
+// What a backward raises: autograd hands a Python exception on as it is, so the caller sees the
+// package's error there too.
+[[noreturn]] void raise_in_backward(const Status& e) {
+  const py::gil_scoped_acquire gil;
+  PyErr_SetObject(error_type().ptr(), error_type()(e.code, e.what()).ptr());
+  python_error raised;
+  raised.persist();
+  throw raised;
 }
 
 void no_second_order(const char* who) {
   // autograd runs a backward in grad mode only to differentiate it again
   if (at::GradMode::is_enabled())
-    throw std::runtime_error(std::string("LMCE_ERR_UNSUPPORTED: ") + who + ": no second derivative (create_graph=True)");
+    throw Status(LMCE_ERR_UNSUPPORTED, std::string(who) + ": no second derivative (create_graph=True)");
 }
 
 // None of these operators has a forward-mode derivative, and the plain path would drop a tangent.
@@ -165,6 +163,14 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    try {
+      return gradients(ctx, grads);
+    } catch (const Status& e) {
+      raise_in_backward(e);
+    }
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     no_second_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor &s = saved[0], &w = saved[1], &rstd = saved[2];
@@ -184,10 +190,10 @@ struct NormNode : torch::autograd::Function<NormNode> {
       const Tensor g = dy.defined() ? rows(dy) : Tensor(), gs = ds.defined() ? rows(ds) : Tensor();
       const size_t need = run_w ? lib.lmce_add_rmsnorm_bwd_workspace_bytes(n, h) : 0;
       if (run_w) ws = bytes(s, need);
-      check_backward(lib.lmce_add_rmsnorm_backward(ptr(g), ptr(gs), s.data_ptr(), w.data_ptr(),
-                                                   static_cast<const float*>(rstd.data_ptr()), n, h,
-                                                   dtype_code(s.scalar_type()), ptr(dx), run_w ? dw.data_ptr() : nullptr,
-                                                   ptr(ws), need, stream(s)));
+      check(lib.lmce_add_rmsnorm_backward(ptr(g), ptr(gs), s.data_ptr(), w.data_ptr(),
+                                          static_cast<const float*>(rstd.data_ptr()), n, h,
+                                          dtype_code(s.scalar_type()), ptr(dx), run_w ? dw.data_ptr() : nullptr,
+                                          ptr(ws), need, stream(s)));
     }
     return {want_x ? dx : Tensor(), want_r ? dx : Tensor(), dw, Tensor()};
   }
@@ -278,6 +284,14 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    try {
+      return gradients(ctx, grads);
+    } catch (const Status& e) {
+      raise_in_backward(e);
+    }
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     no_second_order("gated_linear");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2];
@@ -293,10 +307,10 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
       const Tensor g = rows(grads[0]);
       const size_t need = lib.lmce_gated_bwd_workspace_bytes(n, h, f, want_x, want_g + want_u);
       const Tensor ws = bytes(x, need);
-      check_backward(lib.lmce_gated_backward(g.data_ptr(), saved[3].data_ptr(), x.data_ptr(), wg.data_ptr(),
-                                             wu.data_ptr(), n, h, f, dtype_code(x.scalar_type()),
-                                             static_cast<int>(ctx->saved_data["act"].toInt()), ptr(dx), ptr(dg), ptr(du),
-                                             ws.data_ptr(), need, stream(x)));
+      check(lib.lmce_gated_backward(g.data_ptr(), saved[3].data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(),
+                                    n, h, f, dtype_code(x.scalar_type()),
+                                    static_cast<int>(ctx->saved_data["act"].toInt()), ptr(dx), ptr(dg), ptr(du),
+                                    ws.data_ptr(), need, stream(x)));
       check_device();
     }
     return {dx, dg, du, Tensor()};
@@ -380,11 +394,6 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
   if (rc == LMCE_ERR_INVALID_ARGUMENT) return std::nullopt;  // refused before any launch: shared memory
   check(rc);
   return total;
-}
-
-py::object& error_type() {
-  static py::object* type = new py::object();  // outlives the interpreter's teardown
-  return *type;
 }
 
 void init(const std::string& library, const py::object& error) {

@@ -39,3 +39,16 @@ def test_tangents_are_refused(cuda_device):
             with pytest.raises(_lib.LmceError, match="forward-mode"):
                 call()
     assert (p.grad == 3.0).all()
+
+
+def test_a_backward_raises_the_packages_error(cuda_device):
+    x, r, w, wg, wu = _inputs(cuda_device)
+    x.requires_grad_(True)
+    for out in (add_rms_norm(x, r, w)[0], gated_linear(x, wg, wu)):
+        with pytest.raises(_lib.LmceError, match="second derivative") as e:
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+        assert e.value.code == _lib.LMCE_ERR_UNSUPPORTED
+        loss = out.float().square().sum()
+        with pytest.raises(_lib.LmceError):
+            loss.backward(create_graph=True)
+        assert x.grad is None
