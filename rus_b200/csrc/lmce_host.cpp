@@ -16,7 +16,9 @@
 #include <torch/version.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -99,6 +101,20 @@ void no_tangents(const char* who, std::initializer_list<std::reference_wrapper<c
     if (dual(t)) throw Status(LMCE_ERR_UNSUPPORTED, std::string(who) + ": no forward-mode derivative");
 }
 
+// A tracer sees the allocation of an output, not the kernel that fills it: what it records would
+// return memory as it was found.
+void no_trace(const char* who) {
+  using Key = c10::impl::TorchDispatchModeKey;
+  bool traced = at::tracer::impl::is_dispatch_enabled() ||
+                c10::impl::tls_is_dispatch_key_included(at::DispatchKey::PreDispatch);
+  if (!traced && c10::impl::TorchDispatchModeTLS::any_modes_set())
+    traced = c10::impl::TorchDispatchModeTLS::get_mode(Key::PROXY).has_value() ||
+             c10::impl::TorchDispatchModeTLS::get_mode(Key::FAKE).has_value();
+  if (traced)
+    throw Status(LMCE_ERR_UNSUPPORTED,
+                 std::string(who) + ": cannot be traced (torch.jit.trace, make_fx, torch.export, fake tensors)");
+}
+
 bool is16(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 int dtype_code(at::ScalarType t) { return t == at::kHalf ? LMCE_DTYPE_F16 : LMCE_DTYPE_BF16; }
 
@@ -171,6 +187,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    no_trace("add_rms_norm");
     no_second_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
     const Tensor &s = saved[0], &w = saved[1], &rstd = saved[2];
@@ -205,6 +222,7 @@ bool records(const Tensor& a, const Tensor& b, const std::optional<Tensor>& c) {
 
 std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const std::optional<Tensor>& residual,
                                                        const Tensor& weight, double eps) {
+  no_trace("add_rms_norm");
   no_tangents("add_rms_norm", {x, residual ? *residual : x, weight});
   if (!norm_args(x, residual, weight)) return std::nullopt;
   if (records(x, weight, residual)) {
@@ -218,6 +236,7 @@ std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const st
 std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_e4m3(const Tensor& x,
                                                                     const std::optional<Tensor>& residual,
                                                                     const Tensor& weight, double eps) {
+  no_trace("add_rms_norm_e4m3");
   no_tangents("add_rms_norm_e4m3", {x, residual ? *residual : x, weight});
   if (!norm_args(x, residual, weight) || records(x, weight, residual)) return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
@@ -292,6 +311,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    no_trace("gated_linear");
     no_second_order("gated_linear");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2];
@@ -318,6 +338,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
 };
 
 std::optional<Tensor> gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, int64_t act) {
+  no_trace("gated_linear");
   no_tangents("gated_linear", {x, w_gate, w_up});
   if (!gated_args(x, w_gate, w_up, 64) || !is16(x.scalar_type())) return std::nullopt;
   if (records(x, w_gate, w_up)) return GatedNode::apply(x, w_gate, w_up, act);
@@ -327,6 +348,7 @@ std::optional<Tensor> gated_linear(const Tensor& x, const Tensor& w_gate, const 
 std::optional<Tensor> gated_linear_e4m3(const Tensor& x, const Tensor& x_scale, const Tensor& w_gate,
                                         const Tensor& gate_scale, const Tensor& w_up, const Tensor& up_scale,
                                         int64_t act, at::ScalarType out_dtype) {
+  no_trace("gated_linear_e4m3");
   no_tangents("gated_linear_e4m3", {x, x_scale, w_gate, gate_scale, w_up, up_scale});
   if (!gated_args(x, w_gate, w_up, 128) || x.scalar_type() != at::kFloat8_e4m3fn || !is16(out_dtype))
     return std::nullopt;
@@ -358,6 +380,7 @@ std::optional<Tensor> gated_linear_e4m3(const Tensor& x, const Tensor& x_scale, 
 // fp16, bf16 or fp32 gradients on one device, at least one and none shared. Nothing for any other,
 // and nothing is launched then.
 std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, bool of_parameters) {
+  no_trace("clip_grad_norm_");
   std::vector<void*> ptrs;
   std::vector<int64_t> numels;
   std::vector<int32_t> dtypes;

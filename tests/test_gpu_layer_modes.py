@@ -52,3 +52,49 @@ def test_a_backward_raises_the_packages_error(cuda_device):
         with pytest.raises(_lib.LmceError):
             loss.backward(create_graph=True)
         assert x.grad is None
+
+
+def test_traces_are_refused(cuda_device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, r, w, wg, wu = _inputs(cuda_device)
+    q, sx = _e4m3(x)
+    (g8, sg), (u8, su) = _e4m3(wg), _e4m3(wu)
+
+    def clip(a):
+        p = torch.zeros_like(a, requires_grad=True)
+        p.grad = a
+        return clip_grad_norm_([p], 1.0)
+
+    for f in (lambda a: add_rms_norm(a, r, w), lambda a: add_rms_norm_e4m3(a, None, w),
+              lambda a: gated_linear(a, wg, wu), lambda a: gated_linear_e4m3(q, sx, g8, sg, u8, su),
+              clip):
+        for trace in (lambda: torch.jit.trace(f, (x,), check_trace=False), lambda: make_fx(f)(x),
+                      lambda: make_fx(f, tracing_mode="fake")(x)):
+            with pytest.raises(_lib.LmceError, match="traced"):
+                trace()
+    # the backward alone
+    a = x.clone().requires_grad_(True)
+    for out in (add_rms_norm(a, r, w)[0], gated_linear(a, wg, wu)):
+        with pytest.raises(_lib.LmceError, match="traced"):
+            make_fx(lambda d: torch.autograd.grad(out, a, d))(torch.ones_like(out))
+    # torch.compile leaves these calls to run as they are
+    f = torch.compile(lambda a: add_rms_norm(a * 2, r, w)[0], backend="eager")
+    assert torch.equal(f(x), add_rms_norm(x * 2, r, w)[0])
+
+
+def test_modes_that_watch_see_the_same_results(cuda_device):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    x, r, w, wg, wu = _inputs(cuda_device)
+    a = x.clone().requires_grad_(True)
+
+    def step():
+        y, s = add_rms_norm(a, r, w)
+        h = gated_linear(y, wg, wu)
+        return (h.detach(), *torch.autograd.grad(h.float().sum() + s.float().sum(), a))
+
+    want = step()
+    with FlopCounterMode(display=False):
+        got = step()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

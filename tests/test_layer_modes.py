@@ -41,3 +41,38 @@ def test_tangents_are_refused(name):
             with fwd._set_fwd_grad_enabled(False):  # tangents are not asked for
                 assert call(*bad) is None
         assert call(*args) is None  # no tangent among the arguments: what is wrong here is the device
+
+
+def _refused_as_traced(call, *args):
+    with pytest.raises(_lib.LmceError, match="traced") as e:
+        call(*args)
+    assert e.value.code == _lib.LMCE_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_traces_are_refused(name):
+    """A trace holds the outputs' allocation and not the kernel: it would return memory as found."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    args, _ = _calls()[name]
+    call = getattr(_lib.host(), name)
+    seen = []
+
+    def f(a):
+        _refused_as_traced(call, *args)
+        seen.append(1)
+        return a + 1
+
+    a = torch.ones(3)
+    torch.jit.trace(f, (a,), check_trace=False)
+    make_fx(f)(a)
+    make_fx(f, pre_dispatch=True)(a)
+    make_fx(f, tracing_mode="fake")(a)
+    with FakeTensorMode():
+        f(torch.ones(3))
+    assert len(seen) == 5
+    with FlopCounterMode(display=False):  # a mode that watches what runs
+        assert call(*args) is None
+    assert call(*args) is None
