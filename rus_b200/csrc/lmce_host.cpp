@@ -120,9 +120,12 @@ int dtype_code(at::ScalarType t) { return t == at::kHalf ? LMCE_DTYPE_F16 : LMCE
 
 // `t` contiguous and on a 16-byte boundary (a copy where it is not).
 Tensor rows(const Tensor& t) {
-  if (!t.is_contiguous()) return t.contiguous();
-  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
-  return t.clone(at::MemoryFormat::Contiguous);
+  const Tensor c = t.is_contiguous() ? t : t.contiguous();
+  const void* p = c.data_ptr();
+  // the library would take the null pointer for an argument left out
+  if (p == nullptr && c.numel() > 0)
+    throw Status(LMCE_ERR_UNSUPPORTED, "a tensor that holds no memory (a wrapper of another, or zeros without storage)");
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }

@@ -98,3 +98,18 @@ def test_modes_that_watch_see_the_same_results(cuda_device):
     with FlopCounterMode(display=False):
         got = step()
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_tensors_without_memory_are_refused(cuda_device):
+    """Their null pointer must not read as an argument that was left out."""
+    x, r, w, wg, wu = _inputs(cuda_device)
+    zeros = torch._efficientzerotensor(x.shape, device=cuda_device, dtype=x.dtype)
+    inside = torch.func.functionalize
+    for call in (lambda: add_rms_norm(x, zeros, w), lambda: add_rms_norm_e4m3(x, zeros, w),
+                 lambda: gated_linear(zeros, wg, wu), lambda: inside(lambda t: add_rms_norm(x, t, w)[1])(r),
+                 lambda: inside(lambda t: gated_linear(t, wg, wu))(x)):
+        with pytest.raises(_lib.LmceError, match="no memory") as e:
+            call()
+        assert e.value.code == _lib.LMCE_ERR_UNSUPPORTED
+    for n in (0, 4):  # an empty tensor has a null pointer too
+        assert add_rms_norm(x[:n], x[:n], w)[1].shape == (n, 128)
