@@ -51,9 +51,10 @@ def _clip_any(params: list[torch.Tensor], max_norm: float, error_if_nonfinite: b
         if not torch.isfinite(total):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {total.item()}, nothing was scaled")
     total = run(max_norm)
-    for g, c in zip(grads, flat):
-        if c is not g:
-            g.copy_(c)
+    if max_norm != float("inf"):
+        for g, c in zip(grads, flat):
+            if c is not g:
+                g.copy_(c)
     return total
 
 
@@ -65,11 +66,12 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     skipped, one that is listed twice counts once. Gradients: fp16, bf16 or fp32, mixed, on
     one CUDA device, of any alignment (a non-contiguous one goes through a copy), none
     overlapping another in memory. The norm is over this process's gradients: for a
-    vocabulary shard it covers the shard. They are multiplied by ``max_norm / (norm + 1e-6)`` where that is below 1 and left as they are
-    otherwise; a norm that is not a number makes them all so, an infinite one zeroes the
-    finite ones, as in torch; ``max_norm=inf`` only measures. Nothing is read back to the host
-    unless ``error_if_nonfinite`` asks for an error in those two cases (before any gradient
-    changes)."""
+    vocabulary shard it covers the shard. They are multiplied by ``max_norm / (norm + 1e-6)``
+    where that is below 1 and left as they are otherwise; a norm that is not a number makes
+    them all so, an infinite one zeroes the finite ones, as in torch; ``max_norm=inf`` only
+    measures. With any other limit autograd sees an in-place change of each gradient, scaled or
+    not. Nothing is read back to the host unless ``error_if_nonfinite`` asks for an error in
+    those two cases (before any gradient changes)."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -24,6 +24,7 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <cstdlib>
 #include <functional>
 #include <initializer_list>
@@ -387,11 +388,13 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
   std::vector<void*> ptrs;
   std::vector<int64_t> numels;
   std::vector<int32_t> dtypes;
+  std::vector<at::TensorImpl*> impls;
   Tensor first;
   const size_t count = tensors.size();
   ptrs.reserve(count);
   numels.reserve(count);
   dtypes.reserve(count);
+  impls.reserve(count);
   for (size_t i = 0; i < count; ++i) {
     PyObject* o = PyList_GET_ITEM(tensors.ptr(), static_cast<Py_ssize_t>(i));
     if (!THPVariable_Check(o)) return std::nullopt;
@@ -408,6 +411,7 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
     ptrs.push_back(g.data_ptr());
     numels.push_back(g.numel());
     dtypes.push_back(t == at::kFloat ? LMCE_DTYPE_F32 : dtype_code(t));
+    impls.push_back(g.unsafeGetTensorImpl());
   }
   if (!first.defined()) return std::nullopt;
   const c10::cuda::CUDAGuard guard(first.device());
@@ -419,6 +423,10 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
                                          static_cast<float*>(total.data_ptr()), ws.data_ptr(), need, stream(first));
   if (rc == LMCE_ERR_INVALID_ARGUMENT) return std::nullopt;  // refused before any launch: shared memory
   check(rc);
+  // an in-place change that autograd has to see: a graph that saved a gradient must not use it scaled
+  if (static_cast<float>(max_norm) != INFINITY)
+    for (at::TensorImpl* g : impls)
+      if (!g->is_inference()) g->bump_version();
   return total;
 }
 

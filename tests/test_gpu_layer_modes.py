@@ -113,3 +113,29 @@ def test_tensors_without_memory_are_refused(cuda_device):
         assert e.value.code == _lib.LMCE_ERR_UNSUPPORTED
     for n in (0, 4):  # an empty tensor has a null pointer too
         assert add_rms_norm(x[:n], x[:n], w)[1].shape == (n, 128)
+
+
+def test_clipping_is_an_in_place_change(cuda_device):
+    """Of every gradient, through either path, as torch's own; measuring alone is none."""
+    def param(n, strided=False):
+        p = torch.zeros(n, n, device=cuda_device, requires_grad=True)
+        g = torch.ones(n, n, device=cuda_device)
+        p.grad = g.t().contiguous().t() if strided else g
+        return p
+
+    for strided in (False, True):
+        params = [param(3), param(5, strided)]
+        versions = lambda: [p.grad._version for p in params]  # noqa: E731
+        before = versions()
+        clip_grad_norm_(params, float("inf"))
+        assert versions() == before
+        leaf = torch.ones(5, 5, device=cuda_device, requires_grad=True)
+        kept = (leaf * params[1].grad).sum()  # its backward needs the gradient as it was
+        clip_grad_norm_(params, 1.0)
+        assert all(a > b for a, b in zip(versions(), before))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+    with torch.inference_mode():
+        p = param(4)
+        clip_grad_norm_([p], 1.0)
+        assert abs(p.grad.norm().item() - 1.0) < 1e-5
