@@ -129,6 +129,16 @@ Tensor rows(const Tensor& t) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
 }
 
+// A saved tensor as a hook of torch.autograd.graph.saved_tensors_hooks gives it back: its strides may
+// be others than those that were saved; with another device, type or size it is refused, since the
+// kernels go by those of the gradient.
+Tensor unpacked(const Tensor& t, const Tensor& grad, at::ScalarType type, at::IntArrayRef sizes) {
+  if (!t.defined() || t.layout() != at::kStrided || t.device() != grad.device() || t.scalar_type() != type ||
+      t.sizes() != sizes)
+    throw Status(LMCE_ERR_INVALID_ARGUMENT, "a saved tensor came back with another device, type or size");
+  return rows(t);
+}
+
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 bool usable(const Tensor& t) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided; }
@@ -194,15 +204,18 @@ struct NormNode : torch::autograd::Function<NormNode> {
     no_trace("add_rms_norm");
     no_second_order("add_rms_norm");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &s = saved[0], &w = saved[1], &rstd = saved[2];
     const bool residual = ctx->saved_data["residual"].toBool();
     // edges are counted over the tensors there are
     const bool want_x = ctx->needs_input_grad(0), want_r = residual && ctx->needs_input_grad(1);
     const bool want_w = ctx->needs_input_grad(residual ? 2 : 1);
     const Tensor dy = grads[0], ds = residual ? grads[1] : Tensor();
     if (!dy.defined() && !ds.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const c10::cuda::CUDAGuard guard(s.device());
-    const int64_t n = rstd.numel(), h = s.size(-1);
+    const Tensor& d = dy.defined() ? dy : ds;  // both have the shape and type of s
+    const int64_t h = d.size(-1), n = d.numel() / h;
+    const c10::cuda::CUDAGuard guard(d.device());
+    const Tensor s = unpacked(saved[0], d, d.scalar_type(), d.sizes());
+    const Tensor w = unpacked(saved[1], d, d.scalar_type(), {h});
+    const Tensor rstd = unpacked(saved[2], d, at::kFloat, {n});
     Tensor dx, dw, ws;
     if (want_x || want_r) dx = at::empty_like(s);
     const bool run_w = want_w && dy.defined() && n > 0;
@@ -318,9 +331,12 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     no_trace("gated_linear");
     no_second_order("gated_linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2];
-    const c10::cuda::CUDAGuard guard(x.device());
-    const int64_t f = wg.size(0), h = wg.size(1), n = x.numel() / h;
+    const Tensor& d = grads[0];
+    const c10::cuda::CUDAGuard guard(d.device());
+    const at::ScalarType type = d.scalar_type();
+    const int64_t f = d.size(-1), n = d.numel() / f, h = saved[1].size(-1);
+    const Tensor x = unpacked(saved[0], d, type, out_sizes(d, h));
+    const Tensor wg = unpacked(saved[1], d, type, {f, h}), wu = unpacked(saved[2], d, type, {f, h});
     const bool want_x = ctx->needs_input_grad(0), want_g = ctx->needs_input_grad(1),
                want_u = ctx->needs_input_grad(2);
     const auto make = [&](bool want, const Tensor& like) {
@@ -328,10 +344,12 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     };
     Tensor dx = make(want_x, x), dg = make(want_g, wg), du = make(want_u, wu);
     if (n > 0 && (want_x || want_g || want_u)) {
-      const Tensor g = rows(grads[0]);
+      const Tensor kept =
+          unpacked(saved[3], d, at::kByte, {static_cast<int64_t>(lib.lmce_gated_saved_bytes(n, f))});
+      const Tensor g = rows(d);
       const size_t need = lib.lmce_gated_bwd_workspace_bytes(n, h, f, want_x, want_g + want_u);
       const Tensor ws = bytes(x, need);
-      check(lib.lmce_gated_backward(g.data_ptr(), saved[3].data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(),
+      check(lib.lmce_gated_backward(g.data_ptr(), kept.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(),
                                     n, h, f, dtype_code(x.scalar_type()),
                                     static_cast<int>(ctx->saved_data["act"].toInt()), ptr(dx), ptr(dg), ptr(du),
                                     ws.data_ptr(), need, stream(x)));

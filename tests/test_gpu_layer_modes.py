@@ -139,3 +139,45 @@ def test_clipping_is_an_in_place_change(cuda_device):
         p = param(4)
         clip_grad_norm_([p], 1.0)
         assert abs(p.grad.norm().item() - 1.0) < 1e-5
+
+
+def _strided(t):
+    if t.dim() >= 2:
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    return t.repeat_interleave(2)[::2] if t.dim() == 1 else t
+
+
+def _unaligned(t):
+    out = torch.empty(t.numel() + 1, device=t.device, dtype=t.dtype)[1:].view(t.shape)
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+def test_hooks_of_saved_tensors(cuda_device, residual):
+    """A hook may give back other strides; another device, type or size is refused before any launch."""
+    x, r, w, wg, wu = (t.requires_grad_(True) for t in _inputs(cuda_device, n=40, h=256, f=192))
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    dh = torch.randn(2, 20, 192, device=cuda_device, generator=g).half()
+    leaves = (x, w, wg, wu) + ((r,) if residual else ())
+
+    def graph():
+        y, s = add_rms_norm(x.view(2, 20, 256), r.view(2, 20, 256) if residual else None, w)
+        return (gated_linear(y, wg, wu).float() * dh).sum() + s.float().sum()
+
+    want = torch.autograd.grad(graph(), leaves)
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    for unpack in (_strided, _unaligned, lambda t: t.clone()):
+        with hooks(lambda t: t, unpack):
+            loss = graph()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), want))
+
+    def only(op):  # the operator's own saved tensors
+        for unpack in (lambda t: t.cpu(), lambda t: t.to(torch.float64), lambda t: t[:1], lambda t: t.flatten()[:-1]):
+            with hooks(lambda t: t, unpack):
+                out = op()
+            with pytest.raises(_lib.LmceError, match="came back") as e:
+                torch.autograd.grad(out, x, torch.ones_like(out))
+            assert e.value.code == _lib.LMCE_ERR_INVALID_ARGUMENT
+
+    only(lambda: add_rms_norm(x, r if residual else None, w)[0])
+    only(lambda: gated_linear(x, wg, wu))
