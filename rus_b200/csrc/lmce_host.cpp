@@ -175,7 +175,7 @@ NormOut norm_forward(const Tensor& x, const std::optional<Tensor>& residual, con
   if (keep_rstd) o.rstd = at::empty({n}, xc.options().dtype(at::kFloat));
   if (n > 0)
     check(lib.lmce_add_rmsnorm(xc.data_ptr(), ptr(rc), o.w.data_ptr(), static_cast<float>(eps), n, h,
-                               dtype_code(x.scalar_type()), o.s.data_ptr(), o.y.data_ptr(),
+                               dtype_code(x.scalar_type()), residual ? o.s.data_ptr() : nullptr, o.y.data_ptr(),
                                static_cast<float*>(ptr(o.rstd)), stream(x)));
   return o;
 }
@@ -266,7 +266,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_e4m3(const Tensor
   Tensor s = residual ? at::empty_like(xc) : x;
   if (n > 0)
     check(lib.lmce_add_rmsnorm_e4m3(xc.data_ptr(), ptr(rc), w.data_ptr(), static_cast<float>(eps), n, h,
-                                    dtype_code(x.scalar_type()), s.data_ptr(), q.data_ptr(),
+                                    dtype_code(x.scalar_type()), residual ? s.data_ptr() : nullptr, q.data_ptr(),
                                     static_cast<float*>(scale.data_ptr()), stream(x)));
   return std::make_tuple(q, scale, s);
 }

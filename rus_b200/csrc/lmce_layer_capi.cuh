@@ -72,8 +72,8 @@ int add_norm(const void* x, const void* residual, const void* weight, float eps,
   if (!x || !weight || (residual && !s_out) || !(q ? static_cast<void*>(scale) : y))
     return fail(LMCE_ERR_INVALID_ARGUMENT, "null pointer");
   if (int rc = check_rows(n, h, dtype)) return rc;
-  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(s_out) || !aligned16(y) ||
-      !aligned16(q))
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || (residual && !aligned16(s_out)) ||
+      !aligned16(y) || !aligned16(q))
     return fail(LMCE_ERR_INVALID_ARGUMENT, "misaligned buffers");
   DevInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
@@ -83,7 +83,7 @@ int add_norm(const void* x, const void* residual, const void* weight, float eps,
   p.x = static_cast<const uint4*>(x);
   p.residual = static_cast<const uint4*>(residual);
   p.w = static_cast<const uint4*>(weight);
-  p.s_out = static_cast<uint4*>(s_out);
+  p.s_out = residual ? static_cast<uint4*>(s_out) : nullptr;
   p.y = static_cast<uint4*>(y);
   p.q = static_cast<uint2*>(q);
   p.scale = scale;

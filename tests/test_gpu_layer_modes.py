@@ -181,3 +181,17 @@ def test_hooks_of_saved_tensors(cuda_device, residual):
 
     only(lambda: add_rms_norm(x, r if residual else None, w)[0])
     only(lambda: gated_linear(x, wg, wu))
+
+
+def test_inputs_of_any_alignment_without_a_residual(cuda_device):
+    x, r, w, wg, wu = _inputs(cuda_device, n=24, h=520)
+    wide = torch.zeros(24, 600, device=cuda_device, dtype=x.dtype)
+    wide[:, 3:523] = x
+    others = (_unaligned(x), wide[:, 3:523], _strided(x))
+    assert others[0].data_ptr() % 16 == 2
+    for res, other in ((None, None), (r, _unaligned(r))):
+        want, want8 = add_rms_norm(x, res, w), add_rms_norm_e4m3(x, res, w)
+        for t in others:
+            for got, ref in ((add_rms_norm(t, other, _unaligned(w)), want),
+                             (add_rms_norm_e4m3(t, other, _unaligned(w)), want8)):
+                assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, ref))

@@ -76,3 +76,19 @@ def test_traces_are_refused(name):
     with FlopCounterMode(display=False):  # a mode that watches what runs
         assert call(*args) is None
     assert call(*args) is None
+
+
+@pytest.mark.parametrize("name", ["lmce_add_rmsnorm", "lmce_add_rmsnorm_e4m3"])
+def test_the_sum_is_not_looked_at_without_a_residual(name):
+    """The entries refuse a misaligned s_out only where they would write it: here they go on to the
+    device, or to the next argument that is wrong."""
+    p = 4096  # an aligned address that no refused call reads
+    #       x  residual w  eps   n  h   dt s      y/q    rstd/scale stream
+    args = [p, None, p, 1e-6, 4, 64, 0, p + 2, p + 2, p, None]  # y misaligned
+    entry, lib = getattr(_lib.load(), name), _lib.load()
+    assert entry(*args) == _lib.LMCE_ERR_INVALID_ARGUMENT and b"misaligned" in lib.lmce_last_error()
+    args[1], args[8] = p, p
+    assert entry(*args) == _lib.LMCE_ERR_INVALID_ARGUMENT and b"misaligned" in lib.lmce_last_error()
+    if not torch.cuda.is_available():
+        args[1] = None
+        assert entry(*args) == _lib.LMCE_ERR_CUDA
