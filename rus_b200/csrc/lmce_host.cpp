@@ -379,7 +379,7 @@ std::optional<Tensor> gated_linear_e4m3(const Tensor& x, const Tensor& x_scale, 
     return usable(t) && t.scalar_type() == at::kFloat && t.sizes() == sizes && t.device() == x.device();
   };
   if (!scale_ok(x_scale, x.sizes().slice(0, x.dim() - 1)) || !scale_ok(gate_scale, {f}) || !scale_ok(up_scale, {f}) ||
-      records(x_scale, gate_scale, up_scale))
+      records(x_scale, gate_scale, up_scale) || records(x, w_gate, w_up))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor xc = rows(x), wg = rows(w_gate), wu = rows(w_up);

@@ -68,8 +68,9 @@ def gated_linear_e4m3(x: torch.Tensor, x_scale: torch.Tensor, w_gate: torch.Tens
         w8 = (w.float() / scale[:, None]).to(torch.float8_e4m3fn)
 
     H a multiple of 128, F of 64. Products accumulate in fp32, are scaled there, and the
-    result is rounded once to ``out_dtype`` (fp16 or bf16). No backward: the scales must not
-    require a gradient."""
+    result is rounded once to ``out_dtype`` (fp16 or bf16). No backward: a call that autograd
+    would have to record is refused (an e4m3 ``nn.Parameter`` requires a gradient unless it is
+    made with ``requires_grad=False``)."""
     act = ACTIVATIONS.get(activation)
     if act is not None and x.is_cuda:
         out = (_lib._host or _lib.host()).gated_linear_e4m3(x, x_scale, w_gate, gate_scale, w_up, up_scale, act,

@@ -195,3 +195,19 @@ def test_inputs_of_any_alignment_without_a_residual(cuda_device):
             for got, ref in ((add_rms_norm(t, other, _unaligned(w)), want),
                              (add_rms_norm_e4m3(t, other, _unaligned(w)), want8)):
                 assert all(torch.equal(a.float(), b.float()) for a, b in zip(got, ref))
+
+
+def test_e4m3_operands_that_require_a_gradient(cuda_device):
+    x, r, w, wg, wu = _inputs(cuda_device)
+    args = [*_e4m3(x), *_e4m3(wg), *_e4m3(wu)]
+    want = gated_linear_e4m3(*args)
+    for i in range(6):
+        wanting = args[:i] + [torch.nn.Parameter(args[i])] + args[i + 1:]
+        assert wanting[i].requires_grad
+        with pytest.raises(_lib.LmceError, match="no backward") as e:
+            gated_linear_e4m3(*wanting)
+        assert e.value.code == _lib.LMCE_ERR_UNSUPPORTED
+        with torch.no_grad():
+            assert torch.equal(gated_linear_e4m3(*wanting), want)
+    frozen = [torch.nn.Parameter(t, requires_grad=False) for t in args]
+    assert torch.equal(gated_linear_e4m3(*frozen), want)
