@@ -35,16 +35,12 @@ def _clip_any(params: list[torch.Tensor], max_norm: float, error_if_nonfinite: b
                                  "clip_grad_norm_: an expanded gradient (its elements share memory)")
     # the copies of strided gradients hide from the library what shares memory
     starts = [g.data_ptr() for g in grads if g.numel() > 0]
-    overlap = _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients overlap in memory")
     if len(set(starts)) < len(starts):
-        raise overlap
+        raise _lib.LmceError(_lib.LMCE_ERR_INVALID_ARGUMENT, "clip_grad_norm_: gradients overlap in memory")
     flat = [g.contiguous() for g in grads]
 
     def run(limit):
-        total = _lib.host().clip_grad_norm(flat, limit, False)
-        if total is None:
-            raise overlap
-        return total
+        return _lib.host().clip_grad_norm(flat, limit, False)
 
     if error_if_nonfinite:
         total = run(float("inf"))  # measures only

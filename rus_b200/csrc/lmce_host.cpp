@@ -400,7 +400,7 @@ std::optional<Tensor> gated_linear_e4m3(const Tensor& x, const Tensor& x_scale, 
 
 // The gradients of a list of parameters, or a list of gradients. The common case: dense contiguous
 // fp16, bf16 or fp32 gradients on one device, at least one and none shared. Nothing for any other,
-// and nothing is launched then.
+// and nothing is launched then; what the library says against a list of gradients is raised.
 std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, bool of_parameters) {
   no_trace("clip_grad_norm_");
   std::vector<void*> ptrs;
@@ -439,7 +439,8 @@ std::optional<Tensor> clip_grad_norm(const py::list& tensors, double max_norm, b
   const Tensor ws = bytes(first, need);
   const int rc = lib.lmce_clip_grad_norm(ptrs.data(), numels.data(), dtypes.data(), n, static_cast<float>(max_norm),
                                          static_cast<float*>(total.data_ptr()), ws.data_ptr(), need, stream(first));
-  if (rc == LMCE_ERR_INVALID_ARGUMENT) return std::nullopt;  // refused before any launch: shared memory
+  // refused before any launch: a parameter listed twice, say, which the Python module sorts out
+  if (rc == LMCE_ERR_INVALID_ARGUMENT && of_parameters) return std::nullopt;
   check(rc);
   // an in-place change that autograd has to see: a graph that saved a gradient must not use it scaled
   if (static_cast<float>(max_norm) != INFINITY)

@@ -358,7 +358,8 @@ int lmce_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t
                         float max_norm, float* total_norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (!grads || !numels || !dtypes || !total_norm || !workspace)
     return fail(LMCE_ERR_INVALID_ARGUMENT, "null pointer");
-  if (count <= 0 || count > (1 << 20)) return fail(LMCE_ERR_INVALID_ARGUMENT, "bad count");
+  if (count <= 0 || count > (1 << 20))
+    return fail(LMCE_ERR_INVALID_ARGUMENT, "%lld gradients (need 1 to 2^20)", (long long)count);
   if (!(max_norm >= 0.0f)) return fail(LMCE_ERR_INVALID_ARGUMENT, "max_norm must not be negative");
   if (workspace_bytes < lmce_clip_grad_workspace_bytes(count) || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
     return fail(LMCE_ERR_WORKSPACE, "workspace too small or misaligned");

@@ -211,3 +211,24 @@ def test_e4m3_operands_that_require_a_gradient(cuda_device):
             assert torch.equal(gated_linear_e4m3(*wanting), want)
     frozen = [torch.nn.Parameter(t, requires_grad=False) for t in args]
     assert torch.equal(gated_linear_e4m3(*frozen), want)
+
+
+def test_clipping_says_what_the_library_refuses(cuda_device):
+    empty = torch.zeros(0, device=cuda_device)
+    params = [torch.zeros(0, device=cuda_device, requires_grad=True) for _ in range(2 ** 20 + 1)]
+    for p in params:
+        p.grad = empty
+    with pytest.raises(_lib.LmceError, match=r"1048577 gradients \(need 1 to 2\^20\)"):
+        clip_grad_norm_(params, 1.0)
+    assert clip_grad_norm_(params[:-1], 1.0).item() == 0.0
+    p = torch.zeros(4, device=cuda_device, requires_grad=True)
+    p.grad = torch._efficientzerotensor((4,), device=cuda_device)
+    with pytest.raises(_lib.LmceError, match="null"):
+        clip_grad_norm_([p], 1.0)
+    flat = torch.ones(100, device=cuda_device)
+    a, b = (torch.zeros(60, device=cuda_device, requires_grad=True) for _ in range(2))
+    a.grad, b.grad = flat[:60], flat[40:]
+    for check in (False, True):
+        with pytest.raises(_lib.LmceError, match="overlap"):
+            clip_grad_norm_([a, b], 0.1, error_if_nonfinite=check)
+    assert (flat == 1).all()
