@@ -22,6 +22,7 @@ SOURCES = [CSRC / "lmce_capi.cu"]
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "lmce.h"]
 HOST_PATH = PKG_DIR / "_host.so"
 HOST_DEPS = [CSRC / "lmce_host.cpp", INCLUDE / "lmce.h"]
+HOST_ABI = PKG_DIR / "_host.abi"  # what _host.so was built against
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -90,10 +91,24 @@ def needs_build(out: Path = LIB_PATH, deps: list[Path] = DEPS) -> bool:
     return any(dep.stat().st_mtime > mtime for dep in deps)
 
 
+def host_abi() -> str:
+    """What _host.so is tied to: the installed torch and the interpreter."""
+    import torch
+
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}, {sysconfig.get_platform()}\n"
+
+
+def host_needs_build() -> bool:
+    return (needs_build(HOST_PATH, HOST_DEPS) or not HOST_ABI.exists()
+            or HOST_ABI.read_text(encoding="utf-8") != host_abi())
+
+
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """Compile liblmce.so and _host.so where they are missing or older than their sources."""
-    for out, deps, command in ((LIB_PATH, DEPS, compile_command), (HOST_PATH, HOST_DEPS, host_command)):
-        if not force and not needs_build(out, deps):
+    """Compile liblmce.so and _host.so where they are missing or older than their sources, and
+    _host.so where it was built for another torch or interpreter."""
+    for out, stale, command in ((LIB_PATH, lambda: needs_build(LIB_PATH), compile_command),
+                                (HOST_PATH, host_needs_build, host_command)):
+        if not force and not stale():
             continue
         cmd = command()
         if verbose:
@@ -102,6 +117,8 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         cmd[cmd.index("-o") + 1] = str(tmp)
         subprocess.run(cmd, check=True)
         os.replace(tmp, out)
+        if out == HOST_PATH:
+            HOST_ABI.write_text(host_abi(), encoding="utf-8")
     return LIB_PATH
 
 
