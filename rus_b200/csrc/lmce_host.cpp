@@ -19,6 +19,7 @@
 #include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -69,10 +70,14 @@ void check(int rc) {
   if (rc != LMCE_OK) throw Status(rc, lib.lmce_last_error());
 }
 
-// With LMCE_DEBUG set: wait, and raise what a kernel recorded.
+// With LMCE_DEBUG set: wait for the current stream, which the library's own read of the error word
+// does not when the stream is not the default one, and raise what a kernel recorded. Not while a
+// graph is captured: nothing has run then.
 void check_device() {
   const char* s = std::getenv("LMCE_DEBUG");
   if (s == nullptr || s[0] == '\0' || (s[0] == '0' && s[1] == '\0')) return;
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return;
+  c10::cuda::getCurrentCUDAStream().synchronize();
   const int rc = lib.lmce_device_error(1);
   if (rc != LMCE_OK) throw Status(rc, "reported by a kernel");
 }

@@ -232,3 +232,44 @@ def test_clipping_says_what_the_library_refuses(cuda_device):
         with pytest.raises(_lib.LmceError, match="overlap"):
             clip_grad_norm_([a, b], 0.1, error_if_nonfinite=check)
     assert (flat == 1).all()
+
+
+def test_debug_mode_waits_and_raises_what_a_kernel_recorded(cuda_device, monkeypatch):
+    """With LMCE_DEBUG the call that runs behind the failing kernel raises, on any stream. The kernel here
+    is a bounded wait that nothing satisfies."""
+    x, r, w, wg, wu = _inputs(cuda_device)
+    x.requires_grad_(True)
+    e4m3 = [*_e4m3(x.detach()), *_e4m3(wg), *_e4m3(wu)]
+    dh = torch.ones(4, 64, device=cuda_device, dtype=x.dtype)
+    monkeypatch.setenv("LMCE_DEBUG", "1")
+    _lib.device_error(reset=True)
+    out = gated_linear(x, wg, wu)
+    torch.autograd.grad(out, x, dh, retain_graph=True)
+    gated_linear_e4m3(*e4m3)  # all kernels are loaded now
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        for call in (lambda: gated_linear(x, wg, wu), lambda: gated_linear_e4m3(*e4m3)):
+            with torch.cuda.stream(stream):
+                _lib.call("lmce_selftest_wait_timeout", 200_000_000, stream.cuda_stream)
+                with pytest.raises(_lib.LmceError, match="reported by a kernel") as e:
+                    call()
+                assert e.value.code == _lib.LMCE_ERR_TIMEOUT
+            torch.cuda.synchronize()
+            assert _lib.device_error() == 0  # raised once
+    _lib.call("lmce_selftest_wait_timeout", 200_000_000, torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(_lib.LmceError, match="reported by a kernel") as e:
+        torch.autograd.grad(out, x, dh, retain_graph=True)
+    assert e.value.code == _lib.LMCE_ERR_TIMEOUT
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        captured = gated_linear(x, wg, wu)
+    graph.replay()
+    assert torch.equal(captured, out)
+    for off in ("0", ""):
+        monkeypatch.setenv("LMCE_DEBUG", off)
+        _lib.call("lmce_selftest_wait_timeout", 1_000_000, torch.cuda.current_stream().cuda_stream)
+        torch.autograd.grad(gated_linear(x, wg, wu), x, dh)
+        torch.cuda.synchronize()
+        assert _lib.device_error(reset=True) == _lib.LMCE_ERR_TIMEOUT
