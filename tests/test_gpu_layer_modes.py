@@ -273,3 +273,24 @@ def test_debug_mode_waits_and_raises_what_a_kernel_recorded(cuda_device, monkeyp
         torch.autograd.grad(gated_linear(x, wg, wu), x, dh)
         torch.cuda.synchronize()
         assert _lib.device_error(reset=True) == _lib.LMCE_ERR_TIMEOUT
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_another_device_is_current():
+    """Tensors of one device while another is current: forward, backward and clipping run where the
+    tensors are, on that device's current stream."""
+    def run(dev):
+        x, r, w, wg, wu = (t.requires_grad_(True) for t in _inputs(dev, n=300, h=256, f=192))
+        y, s = add_rms_norm(x, r, w)
+        h = gated_linear(y, wg, wu)
+        (h.float().square().sum() + s.float().sum()).backward()
+        total = clip_grad_norm_([x, r, w, wg, wu], 1.0)
+        with torch.no_grad():
+            q, scale, _ = add_rms_norm_e4m3(x, r, w)
+            h8 = gated_linear_e4m3(q, scale, *_e4m3(wg), *_e4m3(wu))
+        return [t.detach().float().cpu() for t in (y, s, h, x.grad, wg.grad, total, q, scale, h8)]
+
+    with torch.cuda.device(0):
+        want = run(torch.device("cuda", 0))
+        got = run(torch.device("cuda", 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
