@@ -85,6 +85,39 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* f) {
   return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
 }
 
+// A bf16 row whose s w passes fp32 (1e19 and more on both sides) where s rstd w does not: its e4m3
+// output once more, from s rstd w in this order. Each warp goes over the whole row, as it is held, for
+// the largest magnitude: no barrier, which the block's other rows would have to join.
+__device__ __forceinline__ void norm_first(const AddNormParams& p, long long row, int t, float rstd) {
+  const uint4* held = (p.residual ? p.s_out : p.x) + row * p.vec;
+  const auto products = [&](int c, float* v) {
+    float w[8];
+    unpack8<true>(held[c], v);
+    unpack8<true>(__ldg(p.w + c), w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * w[j];
+  };
+  __syncwarp();  // a row of one warp: the other lanes' part of the sum (of more, row_reduce had a barrier)
+  float top = 0.f, v[8];
+#pragma unroll 1
+  for (int c = threadIdx.x & 31; c < p.vec; c += 32) {
+    products(c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float k = 448.0f / top;
+  if (t == 0) p.scale[row] = top / 448.0f;
+#pragma unroll 1
+  for (int c = t; c < p.vec; c += p.threads) {
+    products(c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= k;
+    p.q[row * p.vec + c] = pack8_e4m3(v);
+  }
+}
+
 template <bool BF16, int VPT, bool E4M3>
 __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
   __shared__ float2 red[AN_MAX_WARPS];
@@ -171,6 +204,9 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const AddNormParams p) {
           for (int j = 0; j < 8; ++j) f[i][j] *= k;
           p.q[row * p.vec + c] = pack8_e4m3(f[i]);
         }
+      }
+      if constexpr (BF16) {
+        if (m == INFINITY && rstd > 0.f) norm_first(p, row, t, rstd);
       }
     }
   }

@@ -237,3 +237,24 @@ def test_deterministic_on_streams_and_in_a_graph(cuda_device):
         assert torch.equal(y, want[0]) and torch.equal(s, want[1])
         q2, scale2, _ = add_rms_norm_e4m3(x.detach(), r.detach(), ws)
         assert torch.equal(q.float(), q2.float()) and torch.equal(scale, scale2)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("n,h", [(1, 8), (5, 64), (9, 896), (700, 1000), (300, 4096), (3, 16384)])
+def test_e4m3_where_rows_times_weights_pass_fp32(cuda_device, n, h, residual):
+    """bf16 rows and weights whose product is beyond fp32 (|s w| to 1e45) while s rstd w is not; every
+    third row is an ordinary one. The sum of squares, 16384 * 2.5e31, stays within fp32."""
+    x, r, w, dy, ds = _inputs(cuda_device, n, h, torch.bfloat16, seed=10)
+    large = torch.arange(n, device=cuda_device) % 3 != 1
+    x[large] = (x[large].float() * 1e15).bfloat16()
+    r[large] = (r[large].float() * 1e15).bfloat16()
+    w = (w.float() * torch.where(torch.arange(h, device=cuda_device) % 5 == 2, 1e28, 1e3)).bfloat16()
+    q, scale, s = add_rms_norm_e4m3(x, r if residual else None, w, 1e-5)
+    y_ref = _reference(s, w, dy, ds, 1e-5)[0]
+    top = y_ref.abs().amax(-1) / 448
+    assert (s.double().abs().amax() * w.double().abs().amax()) > 2.0 ** 128
+    _close(scale, top, top * 2 ** -20)
+    _close(q.double() * scale.double()[:, None], y_ref, y_ref.abs() * (2 ** -4 + 2 ** -18) + top[:, None] * 2 ** -10)
+    assert (q.float().abs().amax(-1) == 448).all()
+    y, _ = add_rms_norm(x, r if residual else None, w, 1e-5)
+    _close(y, y_ref, y_ref.abs() * (_half(torch.bfloat16) + 2 ** -20))
