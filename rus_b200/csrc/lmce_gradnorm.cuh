@@ -74,8 +74,7 @@ __device__ __forceinline__ GradSpan grad_span(const GradBatch<MAXT>& b, int i) {
   return s;
 }
 
-// The values of vector v (zeros for elements that are not the tensor's). Returns how many
-// values it holds: 8 or 4.
+// The eight values of a vector; of fp32 the four it holds and four zeros.
 __device__ __forceinline__ void grad_unpack(const uint4& u, int dt, float* f) {
   if (dt == GN_F32) {
     f[0] = __uint_as_float(u.x);

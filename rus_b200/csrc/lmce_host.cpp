@@ -2,9 +2,9 @@
 // nodes of lmce_add_rmsnorm, lmce_gated_linear and their e4m3 forms, and the walk over the
 // gradients of lmce_clip_grad_norm, calling the C ABI of liblmce.so. In C++ because these
 // operators are short: a Python autograd function that does nothing takes 73-91 us a step on the
-// hosts of a B200, where the kernels of a small batch take 15 (one B200, residual norm with
-// backward, 2048 x 1536: 113 us through Python, 73 us here; 392 gradients to clip: 157 us of host
-// work in Python).
+// hosts of a B200, where the kernels of a small batch take 17 (one B200, residual norm with
+// backward, 2048 x 1536: 118 us a call through Python, 80-82 us here; 392 gradients to clip: 157 us
+// of host work in Python, 28 us here).
 //
 // Every function returns nothing where an argument is not one it takes: the Python module
 // then says what is wrong with it (norm.py, gated.py, clip.py). Errors of the library
